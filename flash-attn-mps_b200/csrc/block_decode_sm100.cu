@@ -8,17 +8,22 @@
 // as tcgen05.mma kind::f8f6f4 straight from the codes in shared memory: no
 // code is converted in registers, which bounds a decode that unpacks E4M3 for
 // 16-bit products.
-//   * Q and P become sums of E4M3 parts, part i scaled by 2^(4 i): 2 parts
-//     hold bf16's 8 bits of a query exactly and a probability to 2^-8, 3 parts
-//     f16's 11 bits and 2^-12. The parts are extra columns of the same MMA
-//     (N = 16 is its least width, which 4 columns x 2 parts do not fill).
+//   * Q becomes a sum of E4M3 parts, part i scaled by 2^(4 i): 2 parts hold 8
+//     bits of a query (bf16), 3 parts 12 (f16), for elements down to 2^-14 of
+//     the row's largest; smaller ones to 2^-22 (2^-26) of it. The parts are extra
+//     columns of the same MMA (N = 16 is its least width).
+//   * P becomes a sum of E5M2 parts, part i scaled by 2^(3 i): 3 parts for bf16
+//     hold a probability to 2^-9, as the 16-bit type itself would, 4 for f16 to
+//     2^-12, down to 2^-29 of the tile's largest (20 nats); below that the error
+//     stays under 2^-38 (2^-41) of the largest. The wide exponent matters where
+//     the largest keys add nothing to an output (an attention sink's V row is
+//     close to zero): E4M3 parts, which hold 2^-14, lost such rows.
 //   * Thread t owns key t of the tile: the block scales are one factor and one
 //     addend per thread, t_j = s_j * ks_j + log2(vs_j); the row sum takes
 //     p_j / vs_j (see block_attention.cu).
 //   * P is scaled by the tile's own maximum and O^T read back per tile and
-//     summed in registers (N values per thread): E4M3 holds probabilities down
-//     to 2^-18 of the largest, and relative to the tile rather than to the
-//     running maximum no long tail is lost behind one dominant key.
+//     summed in registers (N values per thread): relative to the tile rather
+//     than to the running maximum no long tail is lost behind one dominant key.
 //
 // Persistent and balanced: the visible tiles of all requests form one list;
 // group g of the G groups takes tiles [g T / G, (g+1) T / G) of it, for each
@@ -76,15 +81,18 @@ using pf::f2unpack;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kBias = 8.f;          // probabilities up to 2^8 (E4M3 ends at 448)
+constexpr float kBias = 15.f;         // probabilities up to 2^15 (E5M2 ends at 57344)
+constexpr float kUnbias = 0x1p-15f;   // 2^-kBias: row sums are kept without it
 constexpr int kKeys = 128;            // keys per tile
 constexpr int kUnitRing = 4;          // unit records in shared memory
 
 __device__ int g_block_decode_timeout;
 
+// NP: parts of a query; a probability has one more.
 template <int NP, int C, int DH>
 struct Shape {
-  static constexpr int N = (NP * C + 15) / 16 * 16;
+  static constexpr int N = (NP * C + 15) / 16 * 16;         // columns of S^T
+  static constexpr int NV = ((NP + 1) * C + 15) / 16 * 16;  // columns of O^T
   static constexpr int CT = C < 8 || C == 16 ? C : 8;     // columns per softmax thread
   static constexpr int WG = C / CT;                       // softmax warpgroups
   static constexpr int kThreads = WG * 128 + 128;
@@ -94,8 +102,8 @@ struct Shape {
   // 8- or 16-byte pieces instead of byte by byte (f16, 32 columns: 1720 -> 900
   // cycles a tile); rows of 32, 64 or 128 bytes, swizzled as wide.
   static constexpr bool kPmn = C >= 8;
-  static constexpr int PW = N <= 32 ? 32 : N <= 64 ? 64 : 128;
-  static constexpr int kQ = N * 128 * DH, kP = kPmn ? kKeys * PW : N * 128;
+  static constexpr int PW = NV <= 32 ? 32 : NV <= 64 ? 64 : 128;
+  static constexpr int kQ = N * 128 * DH, kP = kPmn ? kKeys * PW : NV * 128;
   // CTAs per SM that the shape asks for, and tiles whose scales are kept: a K
   // slot of tile t + kRing comes free only after tile t's scales are read when
   // kRing >= K slots + 2.
@@ -107,7 +115,7 @@ struct Shape {
   static constexpr int kMisc = (kFac + (CT >= 8 ? 96 * CT * WG : 0) + 255) / 256 * 256;
   static constexpr uint32_t cols() {
     uint32_t got = 32;
-    while (got < 2 * N + 2 * N * DH) got *= 2;
+    while (got < 2 * N + 2 * NV * DH) got *= 2;
     return got;
   }
   static constexpr uint32_t kCols = cols();               // tensor memory: S^T and O^T, two buffers each
@@ -134,9 +142,9 @@ __device__ __forceinline__ void mma_f8_ss(uint32_t d, uint64_t a, uint64_t b, ui
       "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
-// E4M3 x E4M3 -> f32; a_mn, b_mn: operand stored MN-major.
-__host__ __device__ constexpr uint32_t f8_idesc(int M, int N, int a_mn, int b_mn) {
-  return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+// E4M3 x E4M3 (b_e5m2: x E5M2) -> f32; a_mn, b_mn: operand stored MN-major.
+__host__ __device__ constexpr uint32_t f8_idesc(int M, int N, int a_mn, int b_mn, int b_e5m2) {
+  return (1u << 4) | ((uint32_t)b_e5m2 << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 // Descriptor of an MN-major tile with rows of W bytes, swizzled over W bytes;
 // the stride of 8-row groups along K is 8 W.
@@ -163,15 +171,16 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&u)[W]) {
                  : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
                  : "r"(taddr));
 }
-// The parts of CT columns of a TMEM row (parts C columns apart) as one value
-// each, two columns to a register pair.
-template <int NP, int C, int CT>
+// The parts of CT columns of a TMEM row (parts C columns apart, each 2^STEP
+// times the one behind it) as one value each, two columns to a register pair.
+template <int NP, int STEP, int C, int CT>
 __device__ __forceinline__ void load_columns(uint32_t taddr, uint64_t (&x)[CT / 2]) {
   uint32_t r[NP][CT];
 #pragma unroll
   for (int part = 0; part < NP; ++part) tmem_ld<CT>(taddr + part * C, r[part]);
   tmem_wait_ld();
-  const uint64_t step = f2pack(0.0625f, 0.0625f);
+  constexpr float kStep = 1.f / (1 << STEP);
+  const uint64_t step = f2pack(kStep, kStep);
   auto two = [&](int part, int c) { return f2pack(__uint_as_float(r[part][c]), __uint_as_float(r[part][c + 1])); };
 #pragma unroll
   for (int c = 0; c < CT; c += 2) {
@@ -192,12 +201,17 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {  // saturating,
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// Two codes times a power of two that f16 holds them with.
-__device__ __forceinline__ float2 from_e4m3x2(uint32_t two, float by = 1.f) {
+__device__ __forceinline__ float2 from_e4m3x2(uint32_t two) {
   const uint32_t h = e4m3x2_to_f16x2(two);
-  const __half2 v = *reinterpret_cast<const __half2*>(&h);
-  return __half22float2(by == 1.f ? v : __hmul2(v, __float2half2_rn(by)));
+  return unpack2<__half>(h);
 }
+__device__ __forceinline__ uint32_t e5m2x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;\n" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// An E5M2 code is the upper byte of the same value in f16.
+__device__ __forceinline__ float2 from_e5m2x2(uint32_t two) { return unpack2<__half>(__byte_perm(two, 0, 0x1404)); }
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, &g_block_decode_timeout));
 }
@@ -248,7 +262,7 @@ __global__ void __launch_bounds__(Shape<NP, C, DH>::kThreads, Shape<NP, C, DH>::
     block_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                         const DecodeArgs a) {
   using Sh = Shape<NP, C, DH>;
-  constexpr int N = Sh::N, NSLOT = Sh::NSLOT, CT = Sh::CT, WG = Sh::WG;
+  constexpr int N = Sh::N, NV = Sh::NV, NPV = NP + 1, NSLOT = Sh::NSLOT, CT = Sh::CT, WG = Sh::WG;
   const BlockAttn& p = a.p;
   const int piece = blockIdx.y;                                   // group of the tile list
   const int kh = blockIdx.x / a.cblocks, cb = blockIdx.x - kh * a.cblocks;
@@ -265,7 +279,7 @@ __global__ void __launch_bounds__(Shape<NP, C, DH>::kThreads, Shape<NP, C, DH>::
   volatile int* rec = reinterpret_cast<volatile int*>(misc + Sh::kRec);      // [kUnitRing][R_WORDS]
   float* colfac = reinterpret_cast<float*>(misc + Sh::kCol);                 // [2][C] scale * log2e * 2^e of the query
   int* col_pos = reinterpret_cast<int*>(misc + Sh::kCol + 8 * C);            // [2][C] query position
-  float4* scales = reinterpret_cast<float4*>(misc + Sh::kScale);             // [kRing][8] {ks, log2 vs, 1 / vs}
+  float4* scales = reinterpret_cast<float4*>(misc + Sh::kScale);             // [kRing][8] {ks, log2 vs, 2^-kBias / vs}
   float* wmax = reinterpret_cast<float*>(misc + Sh::kWmax);                  // [WG][2][4][CT]
   float* sums = reinterpret_cast<float*>(misc + Sh::kSum);                   // [2 units][WG][4][CT]
   float* mrow = reinterpret_cast<float*>(misc + Sh::kMrow);                  // [2 units][C]
@@ -486,7 +500,7 @@ __global__ void __launch_bounds__(Shape<NP, C, DH>::kThreads, Shape<NP, C, DH>::
           // The tile that used this entry 8 tiles ago is done: its K slot came free since.
           if (is_blk) {
             const float s = clamp_scale(vs0);
-            scales[(gt % Sh::kRing) * 8 + lane - 16] = make_float4(clamp_scale(ks0), log2f(s), 1.f / s, 0.f);
+            scales[(gt % Sh::kRing) * 8 + lane - 16] = make_float4(clamp_scale(ks0), log2f(s), kUnbias / s, 0.f);
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(Sh::B_FULL + slot));
@@ -543,7 +557,7 @@ __global__ void __launch_bounds__(Shape<NP, C, DH>::kThreads, Shape<NP, C, DH>::
       if (i % 2 == 1) wait_all(bar(Sh::B_FULL + i % NSLOT), (i / NSLOT) & 1);
   } else if (warp == 4 * WG + 1) {
     // --------------------------------------------------------------------- MMA
-    constexpr uint32_t kQk = f8_idesc(128, N, 0, 0), kPv = f8_idesc(128, N, 1, Sh::kPmn);
+    constexpr uint32_t kQk = f8_idesc(128, N, 0, 0, 0), kPv = f8_idesc(128, NV, 1, Sh::kPmn, 1);
     int gt = 0;
     bool ok = true;
     auto pv = [&](int t) {
@@ -556,7 +570,7 @@ __global__ void __launch_bounds__(Shape<NP, C, DH>::kThreads, Shape<NP, C, DH>::
         for (int hf = 0; hf < DH; ++hf)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            mma_f8_ss(tmem + 2 * N + (t & 1) * (N * DH) + hf * N,
+            mma_f8_ss(tmem + 2 * N + (t & 1) * (NV * DH) + hf * NV,
                       sw128_desc(base + slot * Sh::kItem + hf * (kKeys * 128) + kk * 4096, 16, 1024),
                       Sh::kPmn ? mn_desc<Sh::PW>(base + kOffP + (t & 1) * Sh::kP + kk * 32 * Sh::PW)
                                : sw128_desc(base + kOffP + (t & 1) * Sh::kP + kk * 32, 16, 1024),
@@ -657,7 +671,7 @@ __global__ void __launch_bounds__(Shape<NP, C, DH>::kThreads, Shape<NP, C, DH>::
 #pragma unroll
         for (int hf = 0; hf < DH; ++hf) {
           uint64_t x[CT / 2];
-          load_columns<NP, C, CT>(tmem + 2 * N + (t & 1) * (N * DH) + hf * N + lane_off + c0, x);
+          load_columns<NPV, 3, C, CT>(tmem + 2 * N + (t & 1) * (NV * DH) + hf * NV + lane_off + c0, x);
 #pragma unroll
           for (int c = 0; c < CT; c += 2) {
             uint64_t kf, kg;
@@ -679,7 +693,7 @@ __global__ void __launch_bounds__(Shape<NP, C, DH>::kThreads, Shape<NP, C, DH>::
         float x[CT];
         {
           uint64_t s[CT / 2];
-          load_columns<NP, C, CT>(tmem + (gt & 1) * N + lane_off + c0, s);
+          load_columns<NP, 4, C, CT>(tmem + (gt & 1) * N + lane_off + c0, s);
           const uint64_t ks = f2pack(sc.x, sc.x), add = f2pack(sc.y, sc.y);
 #pragma unroll
           for (int c = 0; c < CT; c += 2) f2unpack(ffma2(s[c / 2], fmul2(ks, pair_at(cf, c)), add), x[c], x[c + 1]);
@@ -746,9 +760,9 @@ __global__ void __launch_bounds__(Shape<NP, C, DH>::kThreads, Shape<NP, C, DH>::
           }
           __syncwarp();
         }
-        // Probabilities: row sums in f32, E4M3 parts into the P^T tile.
-        uint32_t codes[NP][CT / 2];                  // two columns each
-        const uint64_t per_v = f2pack(sc.z, sc.z), sixteen = f2pack(16.f, 16.f);
+        // Probabilities: row sums in f32, E5M2 parts into the P^T tile.
+        uint32_t codes[NPV][CT / 2];                 // two columns each
+        const uint64_t per_v = f2pack(sc.z, sc.z), eight = f2pack(8.f, 8.f), minus = f2pack(-1.f, -1.f);
 #pragma unroll
         for (int c = 0; c < CT; c += 2) {
           uint64_t r, f, g;
@@ -763,13 +777,13 @@ __global__ void __launch_bounds__(Shape<NP, C, DH>::kThreads, Shape<NP, C, DH>::
           uint64_t pp = f2pack(p0, p1);
           l[c / 2] = ffma2(l[c / 2], f, fmul2(pp, fmul2(per_v, g)));
 #pragma unroll
-          for (int part = 0; part < NP; ++part) {
+          for (int part = 0; part < NPV; ++part) {
             f2unpack(pp, p0, p1);
-            const uint32_t code = e4m3x2(p0, p1);
+            const uint32_t code = e5m2x2(p0, p1);
             codes[part][c / 2] = code;
-            if (part + 1 < NP) {  // 16 (p - code), exact
-              const float2 d = from_e4m3x2(code, -16.f);
-              pp = ffma2(pp, sixteen, f2pack(d.x, d.y));
+            if (part + 1 < NPV) {  // 8 (p - code), exact
+              const float2 d = from_e5m2x2(code);
+              pp = fmul2(ffma2(f2pack(d.x, d.y), minus, pp), eight);
             }
           }
         }
@@ -779,7 +793,7 @@ __global__ void __launch_bounds__(Shape<NP, C, DH>::kThreads, Shape<NP, C, DH>::
           constexpr int kChunks = Sh::PW / 16;
           const uint32_t xr = (uint32_t)(key_i / (8 / kChunks)) & (kChunks - 1);
 #pragma unroll
-          for (int part = 0; part < NP; ++part) {
+          for (int part = 0; part < NPV; ++part) {
             const uint32_t at = part * C + c0;
             uint8_t* d = pt + key_i * Sh::PW + (((at >> 4) ^ xr) << 4) + (at & 15);
             uint32_t w[CT / 4];
@@ -791,7 +805,7 @@ __global__ void __launch_bounds__(Shape<NP, C, DH>::kThreads, Shape<NP, C, DH>::
         } else {
           const uint32_t col = ((uint32_t)(key_i >> 4) << 4) + (key_i & 15);
 #pragma unroll
-          for (int part = 0; part < NP; ++part)
+          for (int part = 0; part < NPV; ++part)
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
               const int n0 = part * C + c;
@@ -845,13 +859,13 @@ __global__ void __launch_bounds__(Shape<NP, C, DH>::kThreads, Shape<NP, C, DH>::
           const float mx = fmaxf(m, s);
           if (mx != -INFINITY) {
             f = m == -INFINITY ? 0.f : fast_exp2(m - mx);
-            total = total * f + fast_exp2(s - mx + kBias);
+            total = total * f + fast_exp2(s - mx);
             m = mx;
           }
         }
         const bool none = total == 0.f;
-        const float inv = none ? 0.f : f / total;
-        const float lse = none ? -INFINITY : (m - kBias + log2f(total)) * kLn2;
+        const float inv = none ? 0.f : f * kUnbias / total;
+        const float lse = none ? -INFINITY : (m + log2f(total)) * kLn2;
         const int64_t prow_ = (((int64_t)part_slot * p.c.HK + kh) * a.cblocks + cb) * C + c0 + c;
 #pragma unroll
         for (int hf = 0; hf < DH; ++hf) {

@@ -287,6 +287,14 @@ __device__ __forceinline__ void scale_keys(const float* kfac, uint32_t (&r)[N]) 
     r[i + 3] = __float_as_uint(__uint_as_float(r[i + 3]) * f.w);
   }
 }
+// Log2 of the factor that P carries into its 16-bit type. Over a copy of a
+// block-scaled cache f16 P keeps its 11 bits down to 2^-14 / 2^7 of the running
+// maximum (14.6 nats) rather than 2^-14 (9.7): keys that add nothing to the
+// output (an attention sink's V row is close to zero) may stand that far above the rest. With
+// kRescaleThreshold P stays below 2^15. bf16 has float32's exponents.
+template <bool BF16, bool BLOCK>
+constexpr float kPBias = BLOCK && !BF16 ? 7.f : 0.f;
+
 // Whether a query tile whose window covers key tiles [t0, t1) takes key tile j.
 template <bool BLOCK>
 __device__ __forceinline__ bool takes_tile(const PrefillParams& p, int t0, int t1, int j) {

@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float cap_lim = SOFTCAP ? softcap_poly_limit(cap_in) : -1.f;
       // Running max in log2 units; a sink acts as one extra logit with zero value.
       float m_run = p.sinks ? load_float(p.sinks, p.sink_t, h * p.si0) * 1.4426950408889634f : -INFINITY;
-      float l_run = p.sinks ? 1.f : 0.f;
+      float l_run = p.sinks ? kPBias<BF16, BLOCK> > 0.f ? 128.f : 1.f : 0.f;
       bool began = false;  // an earlier tile of this item is in O
       const float* kfac = nullptr;
       if constexpr (BLOCK) {
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint64_t ls2[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) ls2[i] = f2pack(0.f, 0.f);
-        const uint64_t nmsub2 = f2pack(-msub, -msub);
+        const uint64_t nmsub2 = f2pack(kPBias<BF16, BLOCK> - msub, kPBias<BF16, BLOCK> - msub);
         // kMode 0: scores already scaled or biased; 1: softcap by the
         // polynomial tanh; 2: softcap by the identity. The softcap tile takes
         // one route for the whole warp (cap_poly), so the two loops never mix.
@@ -761,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           bulk_commit();
         }
       }
-      if (row_ok) p.lse[(int64_t)h * p.ls0 + t * p.ls1] = l_run > 0.f ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
+      if (row_ok) p.lse[(int64_t)h * p.ls0 + t * p.ls1] = l_run > 0.f ? (m_run - kPBias<BF16, BLOCK> + log2f(l_run)) * kLn2 : -INFINITY;
     }
     if (lane == 0) bulk_wait_all();  // staged output stores complete before the CTA exits
   }

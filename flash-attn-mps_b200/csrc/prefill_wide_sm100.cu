@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
       const float cap_lim = SOFTCAP ? softcap_poly_limit(cap_in) : -1.f;
       // Running max in log2 units; a sink acts as one extra logit with zero value.
       float m_run = p.sinks ? load_float(p.sinks, p.sink_t, h * p.si0) * 1.4426950408889634f : -INFINITY;
-      float l_run = p.sinks ? 1.f : 0.f;
+      float l_run = p.sinks ? kPBias<BF16, BLOCK> > 0.f ? 128.f : 1.f : 0.f;
       const float* kfac = nullptr;
       if constexpr (BLOCK) {
         if (__ldg(p.kflag)) kfac = p.kfac + ((int64_t)it.b * p.HK + it.kh) * p.kfac_stride;
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
         uint64_t ls2[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) ls2[i] = f2pack(0.f, 0.f);
-        const uint64_t nmsub2 = f2pack(-msub, -msub);
+        const uint64_t nmsub2 = f2pack(kPBias<BF16, BLOCK> - msub, kPBias<BF16, BLOCK> - msub);
         uint32_t pk[BN / 2];
         // kMode 0: plain scores; 1: softcap by the polynomial tanh; 2: softcap
         // by the identity (one route per warp and tile, see cap_poly).
@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
             *reinterpret_cast<uint4*>(orow + (c * 32 + v * 8) * 2) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
         }
       }
-      if (row_ok) p.lse[(int64_t)h * p.ls0 + t * p.ls1] = l_run > 0.f ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
+      if (row_ok) p.lse[(int64_t)h * p.ls0 + t * p.ls1] = l_run > 0.f ? (m_run - kPBias<BF16, BLOCK> + log2f(l_run)) * kLn2 : -INFINITY;
     }
   }
   tc_fence_before();

@@ -6,9 +6,18 @@ The helpers and their tolerances are those of test_gpu_block_cache.py.
 import pytest
 import torch
 
+from test_gpu_alibi import _kernel_names
 from test_gpu_block_cache import run_attention
 
 pytestmark = pytest.mark.gpu
+
+
+def run_prefill(*args, **kw):
+    """run_attention on a call that takes the 16-bit copy and the tcgen05 prefill."""
+    got = []
+    names = _kernel_names(lambda: got.append(run_attention(*args, **kw)))
+    assert not names or any("block_copy_kernel" in n for n in names), names
+    return got[0]
 
 
 def dominant_key(nats, v_code, vs_exp=4):
@@ -40,3 +49,12 @@ def test_dominant_key_without_value(dtype, nats, v_code):
     run_attention([3], [111], 4, 1, 256, 32, 32, dtype, mutate=mutate, q_scale=0.2)
     run_attention([2], [1900], 4, 2, 64, 16, 16, dtype, mutate=mutate, q_scale=0.2, window=100, first=4)
     run_attention([2], [1900], 4, 2, 128, 16, 16, dtype, mutate=mutate, q_scale=0.2, splits=3)
+
+
+@pytest.mark.parametrize("nats", [4, 9, 12, 14])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_dominant_key_without_value_in_prompt_chunks(d, dtype, nats):
+    mutate = dominant_key(nats, 0)
+    run_prefill([130, 260], [170, 300], 32, 2, d, 16, 16, dtype, mutate=mutate, q_scale=0.2)
+    run_prefill([130, 260], [500, 300], 32, 2, d, 16, 16, dtype, mutate=mutate, q_scale=0.2, window=90, first=4, sinks=True)

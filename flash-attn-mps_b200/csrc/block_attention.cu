@@ -11,6 +11,7 @@
 #include <cmath>
 
 #include "block_cache.cuh"
+#include "prefill_common.cuh"
 #include "ptx.cuh"
 
 namespace fab {
@@ -111,20 +112,28 @@ __global__ void __launch_bounds__(128) block_attention_any_kernel(const BlockAtt
 // Every prefill row block and head reads its keys again, so decoding them once
 // (1 byte read, 2 written per element: 30 us for 4 requests of 2500..8192 keys
 // with 8 KV heads of 128, in front of 575 us of prefill at 956 TFLOP/s)
-// turns the call into the 16-bit prefill's compute-bound work. code * scale is
-// exact in both 16-bit types for the powers of two that the append writes (4
-// significant bits; f16 within its range). For other scales K keeps the power
-// of two below its scale and the prefill multiplies the scores by the rest
-// (a flag says so on the device); V is rounded to the 16-bit type, as its
-// products are. Rows in front of a window that share a tile with visible ones
-// are written as zeros, rows in tiles that no query sees not at all.
+// turns the call into the 16-bit prefill's compute-bound work. block_mode_kernel
+// looks at the visible scales of every request and KV head first:
+//   0: code * scale is exact in the 16-bit type (4 significant bits): powers of
+//      two, in f16 up to 2^7 (448 * 2^7 = 57344) and K's from 2^-15 on. What
+//      f16 cannot hold of smaller V is below half its least number, which
+//      outputs are rounded to as well; scales below 2^-60 (a block of zeros has
+//      2^-100) make values that add nothing to a score or output in f16.
+//   1: anything else (an f16 element of 65504 is cached as 256 * 2^8): the copy
+//      holds the codes alone and the prefill takes both scales as the formulas
+//      above do, one factor and one addend per key.
+// Rows in front of a window that share a tile with visible ones are written as
+// zeros, rows in tiles that no query sees not at all.
 struct CopyArgs {
   BlockCache c;
   uint16_t* k; uint16_t* v;          // [requests * max_k, HK, D]
   const int32_t* cu_q; int64_t cq0;
   const int32_t* used; int64_t u0;
   int32_t* cu_out; int32_t* used_out;
-  int32_t* flag; float* kfac; int64_t kfac_stride;   // score factors [requests * HK][stride]
+  int32_t* mode;                                     // [requests * HK]
+  float* kfac; int64_t kfac_stride;                  // mode 1: [requests * HK][3][stride] (AttnParams)
+  int32_t* reset;                                    // the prefill launches' two work counters
+  float per_log2;                                    // raw score units of one log2 unit
   int32_t b0, B, max_k, win, first;
 };
 
@@ -133,6 +142,40 @@ __device__ __forceinline__ uint32_t scaled_pair(uint32_t f16x2, float s) {
   const float2 f = unpack2<__half>(f16x2);
   if constexpr (BF16) return pack2<__nv_bfloat16>(f.x * s, f.y * s);
   else return pack2<__half>(f.x * s, f.y * s);
+}
+
+// First key that a window of the request shows (0 without one).
+__device__ __forceinline__ int window_begin(const CopyArgs& a, int n, int len) {
+  return a.win >= 0 ? max(0, len - n - a.win) : 0;
+}
+
+// Whether the 16-bit copy may hold code * scale (see above).
+template <bool BF16>
+__device__ __forceinline__ bool plain_scale(float s, bool key) {
+  const bool two = (__float_as_uint(s) & 0x7fffffu) == 0;
+  if constexpr (BF16) return two;
+  else return s < 0x1p-60f || (two && s <= 0x1p7f && (!key || s >= 0x1p-15f));
+}
+
+// Mode of a (KV head, request); also clears the work counters.
+template <bool BF16>
+__global__ void __launch_bounds__(256) block_mode_kernel(const CopyArgs a) {
+  const int h = blockIdx.x, lb = blockIdx.y, b = a.b0 + lb;
+  if (h == 0 && lb == 0 && threadIdx.x < 2) a.reset[threadIdx.x] = 0;
+  const BlockCache& c = a.c;
+  const int n = a.cu_q[(b + 1) * a.cq0] - a.cu_q[b * a.cq0];
+  const int len = min(a.used[b * a.u0], a.max_k), lo = window_begin(a, n, len);
+  bool plain = true;
+#pragma unroll 4
+  for (int64_t t = (int64_t)threadIdx.x << c.block_shift; t < len; t += (int64_t)256 << c.block_shift) {
+    const int pg = t + c.block > lo || t < a.first ? block_page(c, b, (int)t) : -1;
+    if (pg < 0) continue;
+    const int blk = ((int)t & (c.page - 1)) >> c.block_shift;
+    plain &= plain_scale<BF16>(clamp_scale(__ldg(c.ksc + (int64_t)pg * c.kc0 + (int64_t)blk * c.kc1 + (int64_t)h * c.kc2)), true) &
+             plain_scale<BF16>(clamp_scale(__ldg(c.vsc + (int64_t)pg * c.vc0 + (int64_t)blk * c.vc1 + (int64_t)h * c.vc2)), false);
+  }
+  plain = __syncthreads_and(plain);
+  if (threadIdx.x == 0) a.mode[(int64_t)lb * c.HK + h] = !plain;
 }
 
 // One CTA: 16 tokens (of one page and scale block) of a request, all KV heads.
@@ -146,8 +189,8 @@ __global__ void __launch_bounds__(256) block_copy_kernel(const CopyArgs a) {
     if (lb == a.B - 1) a.cu_out[a.B] = a.B * a.max_k;
     a.used_out[lb] = max(len, 0);
   }
-  if (t0 >= len || n <= 0) return;
-  const int lo = a.win >= 0 ? max(0, len - n - a.win) : 0;
+  if (t0 >= (len + 127) / 128 * 128 || len <= 0 || n <= 0) return;
+  const int lo = window_begin(a, n, len);
   if (a.win >= 0 && t0 >= (a.first + 127) / 128 * 128 && t0 + 16 <= lo / 128 * 128) return;
   const BlockCache& c = a.c;
   const int pg = block_page(c, b, t0);
@@ -157,28 +200,30 @@ __global__ void __launch_bounds__(256) block_copy_kernel(const CopyArgs a) {
   for (int e = threadIdx.x; e < 16 * per_row; e += 256) {
     const int r = e / per_row, rem = e - r * per_row, h = rem / per_head, d = (rem - h * per_head) * 16;
     const int t = t0 + r;
-    if (t >= len) break;
+    const bool codes = a.mode[(int64_t)lb * c.HK + h];
+    if (t >= len && !codes) break;
     uint4 kv[2];
     float s[2];
-    const bool seen = pg >= 0 && (t >= lo || t < a.first);
+    const bool seen = pg >= 0 && t < len && (t >= lo || t < a.first);
     if (seen) {
       kv[0] = __ldcs(reinterpret_cast<const uint4*>(c.k + (int64_t)pg * c.ks0 + (int64_t)(in + r) * c.ks1 + (int64_t)h * c.ks2 + d));
       kv[1] = __ldcs(reinterpret_cast<const uint4*>(c.v + (int64_t)pg * c.vs0 + (int64_t)(in + r) * c.vs1 + (int64_t)h * c.vs2 + d));
-      s[0] = __ldg(c.ksc + (int64_t)pg * c.kc0 + (int64_t)blk * c.kc1 + (int64_t)h * c.kc2);
-      s[1] = __ldg(c.vsc + (int64_t)pg * c.vc0 + (int64_t)blk * c.vc1 + (int64_t)h * c.vc2);
+      s[0] = clamp_scale(__ldg(c.ksc + (int64_t)pg * c.kc0 + (int64_t)blk * c.kc1 + (int64_t)h * c.kc2));
+      s[1] = clamp_scale(__ldg(c.vsc + (int64_t)pg * c.vc0 + (int64_t)blk * c.vc1 + (int64_t)h * c.vc2));
     } else {
       kv[0] = kv[1] = make_uint4(0, 0, 0, 0);
       s[0] = s[1] = 1.f;
     }
-    // K's power of two; what is left of its scale multiplies the scores.
-    float rest = 1.f;
-    if ((__float_as_uint(s[0]) & 0x7fffffu) && s[0] >= 0x1p-126f && s[0] < INFINITY) {
-      const float two = __uint_as_float(__float_as_uint(s[0]) & 0x7f800000u);
-      rest = s[0] / two;
-      s[0] = two;
-      *a.flag = 1;
+    if (codes) {
+      if (d == 0) {  // also of the last tile's keys past the end, whose zero probabilities they meet
+        float* f = a.kfac + 3 * ((int64_t)lb * c.HK + h) * a.kfac_stride + t;
+        f[0] = s[0];
+        f[a.kfac_stride] = log2f(s[1]) * a.per_log2;
+        f[2 * a.kfac_stride] = pf::kSumUnit / s[1];
+      }
+      if (t >= len) continue;
+      s[0] = s[1] = 1.f;
     }
-    if (d == 0) a.kfac[((int64_t)lb * c.HK + h) * a.kfac_stride + t] = rest;
     const int64_t off = (((int64_t)lb * a.max_k + t) * c.HK + h) * c.D + d;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -204,7 +249,7 @@ enum Route { kAny = 0, kDecode = 1, kPrefill = 2 };
 
 struct Plan {
   int route, splits, reqs;       // reqs: requests per prefill pass
-  size_t bytes, kv_bytes, fac_bytes;  // workspace; one of its 16-bit copies, the score factors
+  size_t bytes, kv_bytes, fac_bytes, len_bytes;  // workspace; one of its 16-bit copies, the keys' scales, offsets and lengths
 };
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
@@ -227,19 +272,20 @@ AttnParams prefill_view(const BlockAttn& p, int reqs) {
   v.causal = p.causal; v.win_l = p.win; v.win_r = -1; v.first = p.first;
   v.max_q = p.max_q; v.max_k = p.max_k; v.splits = 1;
   v.scale = p.scale;
-  v.kflag = reinterpret_cast<const int32_t*>(uintptr_t(256));
+  v.kmode = reinterpret_cast<const int32_t*>(uintptr_t(256));
   return v;
 }
 
 bool prefill_supported(const BlockAttn& p) {
   if (!(p.qt == FA_F16 || p.qt == FA_BF16) || p.max_k < 1 || p.c.D % 16 || p.c.D > 256) return false;
+  if (!(p.scale >= 0x1p-60f)) return false;  // the prefill takes maxima of raw scores
   if (((uintptr_t)p.c.k & 15u) || ((uintptr_t)p.c.v & 15u)) return false;
   for (int64_t s : {p.c.ks0, p.c.ks1, p.c.ks2, p.c.vs0, p.c.vs1, p.c.vs2})
     if (s <= 0 || s % 16) return false;
   return prefill_sm100_supported(prefill_view(p, 1));
 }
 
-// Factors of a (request, KV head): whole key tiles, so that a tile reads its 128.
+// Keys of a (request, KV head) with scales: whole key tiles, so that a tile reads its 128.
 int64_t kfac_stride(const BlockAttn& p) { return ((int64_t)p.max_k + 127) / 128 * 128; }
 
 int launch_prefill(const BlockAttn& p, const Plan& plan, void* workspace, cudaStream_t st) {
@@ -252,16 +298,20 @@ int launch_prefill(const BlockAttn& p, const Plan& plan, void* workspace, cudaSt
     a.v = reinterpret_cast<uint16_t*>(ws + 256 + plan.kv_bytes);
     a.kfac = reinterpret_cast<float*>(ws + 256 + 2 * plan.kv_bytes);
     a.kfac_stride = kfac_stride(p);
-    a.flag = reinterpret_cast<int32_t*>(ws + 128);
+    a.per_log2 = 1.f / (p.scale * kLog2e);
     a.cu_out = reinterpret_cast<int32_t*>(ws + 256 + 2 * plan.kv_bytes + plan.fac_bytes);
     a.used_out = a.cu_out + plan.reqs + 1;
+    a.mode = reinterpret_cast<int32_t*>(ws + 256 + 2 * plan.kv_bytes + plan.fac_bytes + plan.len_bytes);
+    a.reset = reinterpret_cast<int32_t*>(ws);
     a.cu_q = p.cu_q; a.cq0 = p.cq0;
     a.used = p.used; a.u0 = p.u0;
     a.b0 = b0; a.B = n; a.max_k = p.max_k; a.win = p.win; a.first = p.first;
     const dim3 grid((unsigned)((p.max_k + 15) / 16), (unsigned)n);
-    // The prefill's work counter and the flag.
-    cudaError_t e = cudaMemsetAsync(ws, 0, 256, st);
-    if (e != cudaSuccess) return fail(FA_ERR_CUDA, "block-scaled prefill counter reset: %s", cudaGetErrorString(e));
+    const dim3 heads((unsigned)p.c.HK, (unsigned)n);
+    if (p.qt == FA_BF16) block_mode_kernel<true><<<heads, 256, 0, st>>>(a);
+    else block_mode_kernel<false><<<heads, 256, 0, st>>>(a);
+    note_launch();
+    FAB_LAUNCH_CHECK("block-scaled prefill scale launch");
     if (p.qt == FA_BF16) block_copy_kernel<true><<<grid, 256, 0, st>>>(a);
     else block_copy_kernel<false><<<grid, 256, 0, st>>>(a);
     note_launch();
@@ -272,9 +322,12 @@ int launch_prefill(const BlockAttn& p, const Plan& plan, void* workspace, cudaSt
     v.used = a.used_out; v.u0 = 1;
     v.cu_q = p.cu_q + (int64_t)b0 * p.cq0;
     v.scratch = ws;
-    v.kflag = a.flag; v.kfac = a.kfac; v.kfac_stride = a.kfac_stride;
-    const int rc = launch_prefill_sm100(v, st);
-    if (rc) return rc;
+    v.kmode = a.mode; v.kfac = a.kfac; v.kfac_stride = a.kfac_stride;
+    for (int codes = 0; codes < 2; ++codes) {
+      v.codes = codes;
+      const int rc = launch_prefill_sm100(v, st);
+      if (rc) return rc;
+    }
   }
   return FA_OK;
 }
@@ -344,7 +397,7 @@ bool prefill_pays(const BlockAttn& p) {
 }
 
 void make_plan(const BlockAttn& p, Plan* plan) {
-  *plan = Plan{kAny, 1, 0, 0, 0, 0};
+  *plan = Plan{kAny, 1, 0, 0, 0, 0, 0};
   // An explicit number of pieces is a decode plan.
   const bool decode = block_decode_supported(p);
   if (p.splits == 0 && prefill_supported(p) && (!decode || prefill_pays(p))) {
@@ -353,8 +406,9 @@ void make_plan(const BlockAttn& p, Plan* plan) {
     const int64_t rows = (1LL << 30) / p.max_k - 1;
     plan->reqs = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)p.B, kPrefillCopy / (2 * one), rows}));
     plan->kv_bytes = up256((size_t)plan->reqs * one);
-    plan->fac_bytes = up256((size_t)plan->reqs * p.c.HK * kfac_stride(p) * sizeof(float));
-    plan->bytes = 256 + 2 * plan->kv_bytes + plan->fac_bytes + up256((size_t)(2 * plan->reqs + 1) * 4);
+    plan->fac_bytes = up256((size_t)plan->reqs * p.c.HK * 3 * kfac_stride(p) * sizeof(float));
+    plan->len_bytes = up256((size_t)(2 * plan->reqs + 1) * 4);
+    plan->bytes = 256 + 2 * plan->kv_bytes + plan->fac_bytes + plan->len_bytes + up256((size_t)plan->reqs * p.c.HK * 4);
   } else if (decode) {
     plan->route = kDecode;
     plan->splits = block_decode_splits(p);

@@ -57,11 +57,14 @@ struct AttnParams {
   int32_t cp_n, cp_r;
   // Calls over a copy of a block-scaled cache (block_attention.cu; prefill
   // kernels without softcap and ALiBi, null for every call of
-  // fa_attention_fwd): with *kflag != 0 the scores of key t of request b and
-  // KV head h are multiplied by kfac[(b * HK + h) * kfac_stride + t]. Keys
-  // below `first` stay visible behind a left window. The caller has zeroed the
-  // work counter.
-  const int32_t* kflag;
+  // fa_attention_fwd): where kmode[b * HK + h] != 0, K and V of request b and KV
+  // head h are codes without their scales, and kfac + 3 (b * HK + h) kfac_stride
+  // holds per key t its K scale, log2(V scale) in raw score units, and
+  // kSumUnit / (V scale), kfac_stride floats apart. Keys below `first` stay visible
+  // behind a left window. One launch takes the heads with kmode 0, one (codes) the
+  // others, each with its work counter (scratch, scratch + 4 bytes), which the caller
+  // has zeroed.
+  const int32_t* kmode; int32_t codes;
   const float* kfac; int64_t kfac_stride;
   int32_t first;
   int32_t T, B, HQ, HK, DQ, DV, page;

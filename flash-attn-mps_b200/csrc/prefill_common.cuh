@@ -45,9 +45,9 @@ struct PrefillParams {
   int32_t group_reqs;                      // requests per work-order group (their K/V share L2; B: one group)
   int32_t B, HQ, HK, n_pairs, causal, win_l, win_r;
   // BLOCK instantiations: keys below first stay visible behind the left
-  // window; score factors per (request, KV head, key) in use when *kflag != 0.
+  // window; kmode, kfac as in AttnParams.
   int32_t first;
-  const int32_t* kflag;
+  const int32_t* kmode;
   const float* kfac; int64_t kfac_stride;
   float scale, softcap;
 };
@@ -264,9 +264,13 @@ __device__ __forceinline__ void tile_range(int row0, int q_len, int k_len, bool 
   *last = z.hi / BN + 1;
 }
 
+// BLOCK: 0: a call of fa_attention_fwd; 1: over a copy of a block-scaled cache, its
+// (request, KV head)s with kmode 0; 2: those with K and V as codes. (One kernel
+// with both row loops spilled registers in both: 605 -> 634 us of prompts.)
+//
 // With first tokens kept visible an item's key tiles are the first tokens'
 // tiles in front of its window, then the window's from j_first on: tile i.
-template <bool BLOCK, typename I>
+template <int BLOCK, typename I>
 __device__ __forceinline__ int tile_at(const PrefillParams& p, const I& it, int i) {
   if constexpr (BLOCK) {
     const int nf = min((p.first + BN - 1) / BN, it.j_first);
@@ -275,28 +279,70 @@ __device__ __forceinline__ int tile_at(const PrefillParams& p, const I& it, int 
     return it.j_first + i;
   }
 }
-// Multiplies a score row by its keys' factors (kfac at the tile's first key, 16-byte aligned).
+// Keys' scales. Volatile: the loads stay where they stand; lifted to the front of
+// a whole score row they cost its registers.
+__device__ __forceinline__ float4 key_scales4(const float* p) {
+  float4 v;
+  asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint64_t key_scales2(const float* p) {
+  uint64_t v;
+  asm volatile("ld.global.nc.b64 %0, [%1];\n" : "=l"(v) : "l"(p));
+  return v;
+}
+// Scores from codes: a row times its keys' K scales, and their V scales added as
+// exponents, so that P carries them (kfac at the tile's first key, 16-byte aligned).
 template <int N>
-__device__ __forceinline__ void scale_keys(const float* kfac, uint32_t (&r)[N]) {
+__device__ __forceinline__ void scale_keys(const float* kfac, int64_t stride, uint32_t (&r)[N]) {
 #pragma unroll
   for (int i = 0; i < N; i += 4) {
-    const float4 f = __ldg(reinterpret_cast<const float4*>(kfac + i));
-    r[i] = __float_as_uint(__uint_as_float(r[i]) * f.x);
-    r[i + 1] = __float_as_uint(__uint_as_float(r[i + 1]) * f.y);
-    r[i + 2] = __float_as_uint(__uint_as_float(r[i + 2]) * f.z);
-    r[i + 3] = __float_as_uint(__uint_as_float(r[i + 3]) * f.w);
+    const float4 f = key_scales4(kfac + i);
+    const float4 a = key_scales4(kfac + stride + i);
+    r[i] = __float_as_uint(fmaf(__uint_as_float(r[i]), f.x, a.x));
+    r[i + 1] = __float_as_uint(fmaf(__uint_as_float(r[i + 1]), f.y, a.y));
+    r[i + 2] = __float_as_uint(fmaf(__uint_as_float(r[i + 2]), f.z, a.z));
+    r[i + 3] = __float_as_uint(fmaf(__uint_as_float(r[i + 3]), f.w, a.w));
   }
+}
+// Where P carries V scales, the row sum takes p / vs times this: sums of small
+// scales' reciprocals stay finite.
+constexpr float kSumUnit = 0x1p-15f;
+// A row's maximum and sum with the sink's logit, which joins at the end where P
+// carries V scales (it has none); returns what O is to be multiplied by.
+__device__ __forceinline__ float join_sink(float sink, float one, float& m, float& l) {
+  const float mx = fmaxf(m, sink);
+  if (mx == -INFINITY) return 1.f;
+  const float f = m == -INFINITY ? 0.f : exp2f(m - mx);
+  l = l * f + exp2f(sink - mx) * one;
+  m = mx;
+  return f;
 }
 // Log2 of the factor that P carries into its 16-bit type. Over a copy of a
 // block-scaled cache f16 P keeps its 11 bits down to 2^-14 / 2^7 of the running
 // maximum (14.6 nats) rather than 2^-14 (9.7): keys that add nothing to the
 // output (an attention sink's V row is close to zero) may stand that far above the rest. With
 // kRescaleThreshold P stays below 2^15. bf16 has float32's exponents.
-template <bool BF16, bool BLOCK>
+template <bool BF16, int BLOCK>
 constexpr float kPBias = BLOCK && !BF16 ? 7.f : 0.f;
 
+// Whether a launch over a block-scaled cache takes an item.
+template <int BLOCK>
+__device__ __forceinline__ bool takes_head(const PrefillParams& p, int b, int kh) {
+  if constexpr (BLOCK == 0) return true;
+  else return (__ldg(p.kmode + (int64_t)b * p.HK + kh) != 0) == (BLOCK == 2);
+}
+// The launch over codes: whether there is any head for it (it begins while the one
+// in front of it ends).
+__device__ __forceinline__ bool any_codes(const PrefillParams& p) {
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  int any = 0;
+  for (int64_t i = threadIdx.x; i < (int64_t)p.B * p.HK; i += blockDim.x) any |= p.kmode[i];
+  return __syncthreads_or(any);
+}
+
 // Whether a query tile whose window covers key tiles [t0, t1) takes key tile j.
-template <bool BLOCK>
+template <int BLOCK>
 __device__ __forceinline__ bool takes_tile(const PrefillParams& p, int t0, int t1, int j) {
   if constexpr (BLOCK) return t1 > t0 && j < t1 && (j >= t0 || j * BN < p.first);
   else return j >= t0 && j < t1;
@@ -388,6 +434,7 @@ inline int prefill_group_reqs(const AttnParams& p) {
 bool prefill_wide_dims(const AttnParams& p);
 int prefill_wide_supported(const AttnParams& p);
 int launch_prefill_wide(const AttnParams& p, const pf::PrefillParams& pp, cudaStream_t stream);
+int launch_codes(const void* kernel, int grid, int threads, int smem, void** args, cudaStream_t stream);
 int prefill_wide_timeout_flag(bool clear);
 
 }  // namespace fab

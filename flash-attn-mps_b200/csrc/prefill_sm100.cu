@@ -155,11 +155,10 @@ __device__ __forceinline__ Item make_item(const PrefillParams& p, int w) {
 // HDIM: head dim (64 or 128) = number of 64-element swizzle regions x 64.
 // ALIBI: scores minus slope * |q_abs - key|; with SOFTCAP as well, the
 // softcapped score minus the bias (the softcap then runs before the row max).
-// BLOCK: a call over a copy of a block-scaled cache. Keys below p.first stay
-// visible behind the left window (the item's key tiles are then two ranges,
-// tile_at), and scores take their key's factor where the cache's scales are no
-// powers of two.
-template <bool BF16, bool SOFTCAP, int HDIM, bool ALIBI, bool BLOCK = false>
+// BLOCK (prefill_common.cuh): over a copy of a block-scaled cache keys below
+// p.first stay visible behind the left window (the item's key tiles are then two
+// ranges, tile_at).
+template <bool BF16, bool SOFTCAP, int HDIM, bool ALIBI, int BLOCK = 0>
 __global__ void __launch_bounds__(kThreads, 1)
     prefill_sm100_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                          const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to,
@@ -171,6 +170,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kHalves = HDIM / 64;             // 64-element regions per row
   constexpr int kLoadBytes = kHalves * kRegion;      // bytes of one Q tile actually loaded
   constexpr int kKVLoadBytes = kHalves * kKVRegion;  // bytes of one K/V tile actually loaded
+  if constexpr (BLOCK == 2) {
+    if (!any_codes(p)) return;
+  }
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_addr(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       w = __shfl_sync(0xffffffffu, w, 0);
       const bool end = w >= n_work;
       const Item it = make_item(p, end ? 0 : w);
-      if (!end && !it.valid) continue;
+      if (!end && (!it.valid || !takes_head<BLOCK>(p, it.b, it.kh))) continue;
       {
         const uint32_t slot = fwd % NWORK;
         if (fwd >= NWORK && !(ok = warp_wait(bar(B_WEMPTY + slot), ((fwd / NWORK) - 1) & 1))) break;
@@ -453,13 +455,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       // Scores up to this magnitude take the softcap's FMA-pipe polynomial.
       const float cap_lim = SOFTCAP ? softcap_poly_limit(cap_in) : -1.f;
       // Running max in log2 units; a sink acts as one extra logit with zero value.
-      float m_run = p.sinks ? load_float(p.sinks, p.sink_t, h * p.si0) * 1.4426950408889634f : -INFINITY;
-      float l_run = p.sinks ? kPBias<BF16, BLOCK> > 0.f ? 128.f : 1.f : 0.f;
+      // Where P carries V scales the sink, which has none, joins at the end instead.
+      constexpr bool CODES = BLOCK == 2;
+      constexpr float kOne = kPBias<BF16, BLOCK> > 0.f ? 128.f : 1.f;  // P of the running maximum
+      float m_run = p.sinks && !CODES ? load_float(p.sinks, p.sink_t, h * p.si0) * 1.4426950408889634f : -INFINITY;
+      float l_run = p.sinks && !CODES ? kOne : 0.f;
       bool began = false;  // an earlier tile of this item is in O
-      const float* kfac = nullptr;
-      if constexpr (BLOCK) {
-        if (__ldg(p.kflag)) kfac = p.kfac + ((int64_t)it.b * p.HK + it.kh) * p.kfac_stride;
-      }
+      const float* kfac = CODES ? p.kfac + 3 * ((int64_t)it.b * p.HK + it.kh) * p.kfac_stride : nullptr;
       for (int jj = 0; jj < (BLOCK ? it.n_all : n_x); ++jj) {
         const int j = BLOCK ? tile_at<BLOCK>(p, it, jj) : x0 + jj;
         if (BLOCK && !takes_tile<BLOCK>(p, x0, x0 + n_x, j)) continue;
@@ -481,9 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld32_at<96>(tS + 96, r);
         }
         tmem_wait_ld();
-        if constexpr (BLOCK) {
-          if (kfac) scale_keys(kfac + key0, r);
-        }
+        if constexpr (CODES) scale_keys(kfac + key0, p.kfac_stride, r);
         // Softcap route for this tile, uniform over the warp: the polynomial
         // tanh when every raw score of the warp's 32 rows (masked columns
         // included) has |s * scale / cap| <= 3/4, else the identity route.
@@ -636,7 +636,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                   p1 = ex2(x1);
                 }
               }
-              ls2[i & 3] = fadd2(ls2[i & 3], f2pack(p0, p1));
+              if constexpr (CODES)  // p / vs
+                ls2[i & 3] = ffma2(f2pack(p0, p1), key_scales2(kfac + 2 * p.kfac_stride + key0 + c8 * 16 + 2 * i), ls2[i & 3]);
+              else
+                ls2[i & 3] = fadd2(ls2[i & 3], f2pack(p0, p1));
               pk[i] = pack_p<BF16>(p0, p1);
             }
             tmem_st8_at<0>(tS + c8 * 8, pk);
@@ -709,8 +712,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       // of a sequence stores its valid rows directly.
       const bool row_ok = q_row < it.q_len;
       const int64_t t = (int64_t)it.q_begin + q_row;
+      constexpr float kUnit = CODES ? kSumUnit : 1.f;
+      float joined = 1.f;
+      if constexpr (CODES) {
+        if (p.sinks)
+          joined = join_sink(load_float(p.sinks, p.sink_t, h * p.si0) * 1.4426950408889634f, kOne * kUnit, m_run, l_run);
+      }
       const bool have = n_x > 0 && l_run > 0.f;
-      const float inv = have ? vscale / l_run : 0.f;
+      const float inv = have ? vscale * (joined * kUnit) / l_run : 0.f;
       const int wrow0 = (is_b ? it.row_b : it.row_a) + sub * 32;
       const bool staged = wrow0 + 32 <= it.q_len;  // warp-uniform
       uint8_t* stg = gbase + OFF_STAGE + warp * kStageWarpBytes;
@@ -761,7 +770,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           bulk_commit();
         }
       }
-      if (row_ok) p.lse[(int64_t)h * p.ls0 + t * p.ls1] = l_run > 0.f ? (m_run - kPBias<BF16, BLOCK> + log2f(l_run)) * kLn2 : -INFINITY;
+      if (row_ok) p.lse[(int64_t)h * p.ls0 + t * p.ls1] = l_run > 0.f ? (m_run - kPBias<BF16, BLOCK> + log2f(l_run / kUnit)) * kLn2 : -INFINITY;
     }
     if (lane == 0) bulk_wait_all();  // staged output stores complete before the CTA exits
   }
@@ -797,7 +806,7 @@ int prefill_sm100_supported(const AttnParams& p) {
       if (v <= 0 || (v * 2) % 16 != 0) return 0;
   }
   if (p.mask || p.leftpad || p.cp_n > 1) return 0;
-  if (p.kflag && (p.softcap > 0.f || p.alibi)) return 0;
+  if (p.kmode && (p.softcap > 0.f || p.alibi)) return 0;
   if (p.sinks && !(p.sink_t == FA_F32 || p.sink_t == FA_F16 || p.sink_t == FA_BF16)) return 0;
   if (p.qs2 != 1 || p.ks3 != 1 || p.vs3 != 1 || p.os2 != 1) return 0;
   if (!al16(p.q) || !al16(p.k) || !al16(p.v) || !al16(p.out)) return 0;
@@ -823,6 +832,24 @@ int prefill_timeout_flag(bool clear) {
   return v | w;
 }
 
+// The launch over codes may begin before the one in front of it ends and waits for it (any_codes).
+int launch_codes(const void* kernel, int grid, int threads, int smem, void** args, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelExC(&cfg, kernel, args);
+  if (e != cudaSuccess) return fail(FA_ERR_CUDA, "prefill launch over codes: %s", cudaGetErrorString(e));
+  note_launch();
+  return FA_OK;
+}
+
 int launch_prefill_sm100(const AttnParams& p, cudaStream_t stream) {
   if (p.T <= 0) return fail(FA_ERR_INVALID, "prefill needs query rows");
   if (!p.paged && p.k_rows <= 0) return fail(FA_ERR_INVALID, "prefill needs packed K/V rows");
@@ -838,7 +865,7 @@ int launch_prefill_sm100(const AttnParams& p, cudaStream_t stream) {
   pp.cu_k = p.cu_k; pp.ck0 = p.ck0;
   pp.used = p.used; pp.u0 = p.u0;
   pp.B = p.B; pp.HQ = p.HQ; pp.HK = p.HK;
-  pp.counter = reinterpret_cast<int*>(p.scratch);
+  pp.counter = p.scratch ? reinterpret_cast<int*>(p.scratch) + (p.kmode && p.codes) : nullptr;
   if (p.paged) {
     pp.table = p.table; pp.bt0 = p.bt0; pp.bt1 = p.bt1;
     pp.bt_cols = (int32_t)p.bt_cols; pp.page_shift = page_shift; pp.box_rows = box_rows;
@@ -855,7 +882,7 @@ int launch_prefill_sm100(const AttnParams& p, cudaStream_t stream) {
   pp.vd = p.vd; pp.vd0 = p.vd0; pp.vd1 = p.vd1;
   pp.win_l = p.win_l; pp.win_r = p.win_r;
   pp.first = p.win_l >= 0 ? p.first : 0;
-  pp.kflag = p.kflag; pp.kfac = p.kfac; pp.kfac_stride = p.kfac_stride;
+  pp.kmode = p.kmode; pp.kfac = p.kfac; pp.kfac_stride = p.kfac_stride;
   pp.scale = p.scale;
   pp.softcap = p.softcap;
   pp.alibi = p.alibi; pp.al0 = p.a0; pp.al1 = p.a1;
@@ -881,8 +908,10 @@ int launch_prefill_sm100(const AttnParams& p, cudaStream_t stream) {
   const bool cap = p.softcap > 0.f, alibi = p.alibi != nullptr;
   auto pick = [&](auto hd) {
     constexpr int H = decltype(hd)::value;
-    if (pp.kflag)
-      return p.qt == FA_BF16 ? prefill_sm100_kernel<true, false, H, false, true> : prefill_sm100_kernel<false, false, H, false, true>;
+    if (pp.kmode && p.codes)
+      return p.qt == FA_BF16 ? prefill_sm100_kernel<true, false, H, false, 2> : prefill_sm100_kernel<false, false, H, false, 2>;
+    if (pp.kmode)
+      return p.qt == FA_BF16 ? prefill_sm100_kernel<true, false, H, false, 1> : prefill_sm100_kernel<false, false, H, false, 1>;
     if (p.qt == FA_BF16)
       return cap ? (alibi ? prefill_sm100_kernel<true, true, H, true> : prefill_sm100_kernel<true, true, H, false>)
                  : alibi ? prefill_sm100_kernel<true, false, H, true> : prefill_sm100_kernel<true, false, H, false>;
@@ -903,8 +932,12 @@ int launch_prefill_sm100(const AttnParams& p, cudaStream_t stream) {
   const int64_t n_work = (int64_t)pp.n_pairs * (p.HQ >> pp.head_pairs) * p.B;
   const int grid = (int)std::min<int64_t>(n_work, (int64_t)sm_count());
   if (pp.counter == nullptr) return fail(FA_ERR_INVALID, "prefill needs its workspace counter");
-  if (!p.kflag) e = cudaMemsetAsync(pp.counter, 0, sizeof(int), stream);
+  if (!p.kmode) e = cudaMemsetAsync(pp.counter, 0, sizeof(int), stream);
   if (e != cudaSuccess) return fail(FA_ERR_CUDA, "prefill counter reset: %s", cudaGetErrorString(e));
+  if (p.kmode && p.codes) {
+    void* args[] = {&mq, &mk, &mv, &mo, &pp};
+    return launch_codes(reinterpret_cast<void*>(kernel), grid, kThreads, kSmemBytes, args, stream);
+  }
   kernel<<<grid, kThreads, kSmemBytes, stream>>>(mq, mk, mv, mo, pp);
   note_launch();
   FAB_LAUNCH_CHECK("prefill launch");

@@ -148,13 +148,16 @@ __device__ __forceinline__ void load_kv_tile(const PrefillParams& p, const Item&
 
 // DQK / DV: padded QK and V head dims (multiples of 64); the tensor maps
 // carry the true dims, so padded columns load as zeros and are never stored.
-// BLOCK: a call over a copy of a block-scaled cache (first tokens, key factors).
-template <bool BF16, bool SOFTCAP, int DQK, int DV, bool BLOCK = false>
+// BLOCK: prefill_common.cuh.
+template <bool BF16, bool SOFTCAP, int DQK, int DV, int BLOCK = 0>
 __global__ void __launch_bounds__(kWThreads, 1)
     prefill_wide_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                         const __grid_constant__ CUtensorMap tv, const PrefillParams p) {
   using L = WideLayout<DQK, DV>;
   constexpr int RQ = L::RQ, RV = L::RV;
+  if constexpr (BLOCK == 2) {
+    if (!any_codes(p)) return;
+  }
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_addr(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -213,7 +216,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
       w = __shfl_sync(0xffffffffu, w, 0);
       const bool end = w >= n_work;
       const Item it = make_wide_item(p, end ? 0 : w);
-      if (!end && !it.valid) continue;
+      if (!end && (!it.valid || !takes_head<BLOCK>(p, it.b, it.kh))) continue;
       {
         const uint32_t slot = fwd % NWORK;
         if (fwd >= NWORK && !(ok = wwait(bar(W_WEMPTY + slot), ((fwd / NWORK) - 1) & 1))) break;
@@ -382,12 +385,12 @@ __global__ void __launch_bounds__(kWThreads, 1)
       // Scores up to this magnitude take the softcap's FMA-pipe polynomial.
       const float cap_lim = SOFTCAP ? softcap_poly_limit(cap_in) : -1.f;
       // Running max in log2 units; a sink acts as one extra logit with zero value.
-      float m_run = p.sinks ? load_float(p.sinks, p.sink_t, h * p.si0) * 1.4426950408889634f : -INFINITY;
-      float l_run = p.sinks ? kPBias<BF16, BLOCK> > 0.f ? 128.f : 1.f : 0.f;
-      const float* kfac = nullptr;
-      if constexpr (BLOCK) {
-        if (__ldg(p.kflag)) kfac = p.kfac + ((int64_t)it.b * p.HK + it.kh) * p.kfac_stride;
-      }
+      // Where P carries V scales the sink, which has none, joins at the end instead.
+      constexpr bool CODES = BLOCK == 2;
+      constexpr float kOne = kPBias<BF16, BLOCK> > 0.f ? 128.f : 1.f;  // P of the running maximum
+      float m_run = p.sinks && !CODES ? load_float(p.sinks, p.sink_t, h * p.si0) * 1.4426950408889634f : -INFINITY;
+      float l_run = p.sinks && !CODES ? kOne : 0.f;
+      const float* kfac = CODES ? p.kfac + 3 * ((int64_t)it.b * p.HK + it.kh) * p.kfac_stride : nullptr;
       for (int jj = 0; jj < n_x; ++jj) {
         const int j = BLOCK ? tile_at<BLOCK>(p, it, jj) : x0 + jj;
         if (!(ok = wwait(bar(W_SF), s_cnt & 1))) break;
@@ -402,9 +405,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
         tmem_ld32_at<64>(tS + 64, r);
         tmem_ld32_at<96>(tS + 96, r);
         tmem_wait_ld();
-        if constexpr (BLOCK) {
-          if (kfac) scale_keys(kfac + key0, r);
-        }
+        if constexpr (CODES) scale_keys(kfac + key0, p.kfac_stride, r);
         // S is in registers: the MMA warp may compute the next scores into it.
         tc_fence_before();
         __syncwarp();
@@ -482,7 +483,10 @@ __global__ void __launch_bounds__(kWThreads, 1)
               p0 = ex2(x0);
               p1 = ex2(x1);
             }
-            ls2[i & 3] = fadd2(ls2[i & 3], f2pack(p0, p1));
+            if constexpr (CODES)  // p / vs
+              ls2[i & 3] = ffma2(f2pack(p0, p1), key_scales2(kfac + 2 * p.kfac_stride + key0 + 2 * i), ls2[i & 3]);
+            else
+              ls2[i & 3] = fadd2(ls2[i & 3], f2pack(p0, p1));
             pk[i] = pack_p<BF16>(p0, p1);
           }
         };
@@ -549,8 +553,14 @@ __global__ void __launch_bounds__(kWThreads, 1)
       // time from tensor memory).
       const bool row_ok = q_row < it.q_len;
       const int64_t t = (int64_t)it.q_begin + q_row;
+      constexpr float kUnit = CODES ? kSumUnit : 1.f;
+      float joined = 1.f;
+      if constexpr (CODES) {
+        if (p.sinks)
+          joined = join_sink(load_float(p.sinks, p.sink_t, h * p.si0) * 1.4426950408889634f, kOne * kUnit, m_run, l_run);
+      }
       const bool have = n_x > 0 && l_run > 0.f;
-      const float inv = have ? vscale / l_run : 0.f;
+      const float inv = have ? vscale * (joined * kUnit) / l_run : 0.f;
       uint8_t* orow = reinterpret_cast<uint8_t*>(p.out) + (t * p.os0 + (int64_t)h * p.os1) * 2;
 #pragma unroll
       for (int c = 0; c < DV / 32; ++c) {
@@ -570,7 +580,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
             *reinterpret_cast<uint4*>(orow + (c * 32 + v * 8) * 2) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
         }
       }
-      if (row_ok) p.lse[(int64_t)h * p.ls0 + t * p.ls1] = l_run > 0.f ? (m_run - kPBias<BF16, BLOCK> + log2f(l_run)) * kLn2 : -INFINITY;
+      if (row_ok) p.lse[(int64_t)h * p.ls0 + t * p.ls1] = l_run > 0.f ? (m_run - kPBias<BF16, BLOCK> + log2f(l_run / kUnit)) * kLn2 : -INFINITY;
     }
   }
   tc_fence_before();
@@ -588,6 +598,12 @@ void* pick_wide(bool bf16, bool cap) {
                : reinterpret_cast<void*>(prefill_wide_kernel<true, false, DQK, DV>);
   return cap ? reinterpret_cast<void*>(prefill_wide_kernel<false, true, DQK, DV>)
              : reinterpret_cast<void*>(prefill_wide_kernel<false, false, DQK, DV>);
+}
+
+template <int DQK, int BLOCK>
+void* pick_block(bool bf16) {
+  return bf16 ? reinterpret_cast<void*>(prefill_wide_kernel<true, false, DQK, 256, BLOCK>)
+              : reinterpret_cast<void*>(prefill_wide_kernel<false, false, DQK, 256, BLOCK>);
 }
 
 }  // namespace
@@ -636,17 +652,11 @@ int launch_prefill_wide(const AttnParams& p, const PrefillParams& pp_in, cudaStr
   const bool bf16 = p.qt == FA_BF16, cap = p.softcap > 0.f;
   void* kernel;
   int smem;
-  if (pp.kflag) {
+  if (pp.kmode) {
     // (192, 256) and (256, 256) also take narrower values.
-    if (p.DQ <= 192) {
-      kernel = bf16 ? reinterpret_cast<void*>(prefill_wide_kernel<true, false, 192, 256, true>)
-                    : reinterpret_cast<void*>(prefill_wide_kernel<false, false, 192, 256, true>);
-      smem = WideLayout<192, 256>::kSmem;
-    } else {
-      kernel = bf16 ? reinterpret_cast<void*>(prefill_wide_kernel<true, false, 256, 256, true>)
-                    : reinterpret_cast<void*>(prefill_wide_kernel<false, false, 256, 256, true>);
-      smem = WideLayout<256, 256>::kSmem;
-    }
+    kernel = p.DQ <= 192 ? p.codes ? pick_block<192, 2>(bf16) : pick_block<192, 1>(bf16)
+                         : p.codes ? pick_block<256, 2>(bf16) : pick_block<256, 1>(bf16);
+    smem = p.DQ <= 192 ? WideLayout<192, 256>::kSmem : WideLayout<256, 256>::kSmem;
   } else if (p.DQ <= 192) {
     if (p.DV <= 128) { kernel = pick_wide<192, 128>(bf16, cap); smem = WideLayout<192, 128>::kSmem; }
     else { kernel = pick_wide<192, 256>(bf16, cap); smem = WideLayout<192, 256>::kSmem; }
@@ -659,9 +669,10 @@ int launch_prefill_wide(const AttnParams& p, const PrefillParams& pp_in, cudaStr
   const int64_t n_work = (int64_t)pp.n_pairs * p.HQ * p.B;
   const int grid = (int)std::min<int64_t>(n_work, (int64_t)sm_count());
   if (pp.counter == nullptr) return fail(FA_ERR_INVALID, "prefill needs its workspace counter");
-  if (!p.kflag) e = cudaMemsetAsync(pp.counter, 0, sizeof(int), stream);
+  if (!p.kmode) e = cudaMemsetAsync(pp.counter, 0, sizeof(int), stream);
   if (e != cudaSuccess) return fail(FA_ERR_CUDA, "prefill counter reset: %s", cudaGetErrorString(e));
   void* args[] = {&mq, &mk, &mv, &pp};
+  if (p.kmode && p.codes) return launch_codes(kernel, grid, kWThreads, smem, args, stream);
   e = cudaLaunchKernel(kernel, dim3(grid), dim3(kWThreads), args, smem, stream);
   note_launch();
   if (e != cudaSuccess) return fail(FA_ERR_CUDA, "wide prefill launch: %s", cudaGetErrorString(e));

@@ -3,9 +3,11 @@
 The helpers and their tolerances are those of test_gpu_block_cache.py.
 """
 
+import numpy as np
 import pytest
 import torch
 
+import test_gpu_block_cache as base
 from test_gpu_alibi import _kernel_names
 from test_gpu_block_cache import run_attention
 
@@ -58,3 +60,73 @@ def test_dominant_key_without_value_in_prompt_chunks(d, dtype, nats):
     mutate = dominant_key(nats, 0)
     run_prefill([130, 260], [170, 300], 32, 2, d, 16, 16, dtype, mutate=mutate, q_scale=0.2)
     run_prefill([130, 260], [500, 300], 32, 2, d, 16, 16, dtype, mutate=mutate, q_scale=0.2, window=90, first=4, sinks=True)
+
+
+@pytest.fixture
+def infinite_past_half(monkeypatch):
+    """Elements whose exact value rounds to f16's infinity: checked to be that, then taken as exact by run_attention."""
+    exact = base.ob.attention
+    call = base.flash_attn_with_block_scaled_kvcache
+
+    def checked(q, kc, vc, ks, vs, used, table, **kw):
+        out, lse = call(q, kc, vc, ks, vs, used, table, **kw)
+        if out.dtype == torch.float16:
+            want = exact(base.np_of(q), [base.np_of(kc), base.np_of(vc)], [base.np_of(ks), base.np_of(vs)], used.tolist(),
+                         base.np_of(table), base.np_of(kw["cu_seqlens_q"]), q.shape[-1] ** -0.5, kw["causal"],
+                         kw["window_size"][0], kw["first_tokens"])[0]
+            got = out.double().cpu().numpy()
+            past = np.abs(want) >= 65520.0 * (1 + 2.0 ** -9)
+            assert np.array_equal(got[past], np.sign(want[past]) * np.inf)
+            near = (np.abs(want) >= 65520.0 * (1 - 2.0 ** -9)) & np.isinf(got) & (np.sign(got) == np.sign(want))
+            out = FloatOut(out, torch.from_numpy(np.where(past | near, want, got)))
+        return out, lse
+    monkeypatch.setattr(base, "flash_attn_with_block_scaled_kvcache", checked)
+
+
+class FloatOut:
+    """An output with some elements replaced in 64 bits."""
+
+    def __init__(self, out, values):
+        self.dtype, self.shape, self.values = out.dtype, out.shape, values
+
+    def double(self):
+        return self.values
+
+
+@pytest.mark.parametrize("k_exp,v_exp", [(-8, 8), (8, 8), (10, 10), (-22, -22), (12, 40)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_scales_beyond_half_precision(dtype, k_exp, v_exp, infinite_past_half):
+    """Blocks whose values leave f16's range (an f16 element of 65504 is cached as 256 * 2^8) or its normal numbers."""
+    def mutate(q, kc, vc, ks, vs, table):
+        for b in range(table.shape[0]):
+            page = table[b, 1].long()
+            ks[page] = 2.0 ** k_exp
+            vs[page] = 2.0 ** v_exp
+            if v_exp > 16:                               # of little weight, so that outputs stay finite
+                kc.view(torch.uint8)[page] = 0
+                kc.view(torch.uint8)[page, :, :, 0] = 0xfe   # -448: a logit of -60 * log(2)
+                q[:, :, 0] = 41.6 * q.shape[-1] ** 0.5 / (448 * 2.0 ** k_exp)
+                vc.view(torch.uint8)[page] &= 0x81
+    q_scale = 2.0 ** -12 if k_exp >= 8 else 1.0
+    for ns in ([1, 1], [4, 3]):
+        run_attention(ns, [170, 300], 8, 2, 128, 16, 16, dtype, mutate=mutate, q_scale=q_scale)
+    for d in (64, 128, 256):
+        run_prefill([130, 260], [170, 300], 32, 2, d, 16, 16, dtype, mutate=mutate, q_scale=q_scale)
+    run_prefill([130, 260], [500, 300], 32, 2, 128, 32, 32, dtype, mutate=mutate, q_scale=q_scale, window=60, first=40)
+
+
+@pytest.mark.parametrize("d", [48, 64, 128, 192, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prompt_chunks_over_any_scales(dtype, d):
+    """Scales that are no powers of two on some KV heads and requests only, blocks of zeros, sinks, first tokens, no causality."""
+    def mutate(q, kc, vc, ks, vs, table):
+        ks[:, :, 1] *= 1.3                                # one KV head everywhere
+        vs[table[1, :2].long(), :, 0] *= 0.77
+        for cache, scale in ((kc, ks), (vc, vs)):            # a block of zeros as the append leaves it
+            cache.view(torch.uint8)[table[0, 2].long()] = 0
+            scale[table[0, 2].long()] = 2.0 ** -100
+    args = [130, 260, 0, 9], [171, 300, 40, 9], 32, 4, d, 16, 16, dtype
+    run_prefill(*args, mutate=mutate)
+    run_prefill(*args, mutate=mutate, sinks=True, window=70, first=20)
+    run_prefill(*args, mutate=mutate, sinks=True, causal=False)
+    run_prefill([130, 260], [20, 300], 32, 4, d, 16, 16, dtype, mutate=mutate, sinks=True)     # rows that see nothing

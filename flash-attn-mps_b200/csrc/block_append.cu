@@ -81,17 +81,21 @@ __global__ void __launch_bounds__(256) block_append_any_kernel(const AppendArgs 
   if (n <= 0) return;
   const int start = a.lens[b * a.l0];
   if (a.q && blockIdx.z == 2) {
-    // Rotated queries of this request.
-    const int D = a.c.D;
-    const int64_t total = (int64_t)n * a.HQ * D, step = (int64_t)gridDim.x * blockDim.x;
+    // Rotated queries of this request: a thread forms both elements of a pair
+    // before it writes them (query_out may be query), the rest one by one.
+    const int per_row = a.c.D - a.half;
+    const int64_t total = (int64_t)n * a.HQ * per_row, step = (int64_t)gridDim.x * blockDim.x;
     for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += step) {
-      const int d = (int)(e % D);
-      const int64_t r = e / D;
+      const int i = (int)(e % per_row);
+      const int64_t r = e / per_row;
       const int h = (int)(r % a.HQ);
       const int j = (int)(r / a.HQ);
-      const int64_t t = begin + j;
-      store_float(a.qo, a.qt, t * a.qo0 + h * a.qo1 + d * a.qo2,
-                  rotated(a, a.q, a.qt, t * a.qs0 + h * a.qs1, a.qs2, d, t, start + j));
+      const int64_t t = begin + j, src = t * a.qs0 + h * a.qs1, dst = t * a.qo0 + h * a.qo1;
+      const int d0 = i >= a.half ? i + a.half : a.interleaved ? 2 * i : i, d1 = a.interleaved ? d0 + 1 : d0 + a.half;
+      const float x0 = rotated(a, a.q, a.qt, src, a.qs2, d0, t, start + j);
+      const float x1 = i < a.half ? rotated(a, a.q, a.qt, src, a.qs2, d1, t, start + j) : 0.f;
+      store_float(a.qo, a.qt, dst + d0 * a.qo2, x0);
+      if (i < a.half) store_float(a.qo, a.qt, dst + d1 * a.qo2, x1);
     }
     return;
   }

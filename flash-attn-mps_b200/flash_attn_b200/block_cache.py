@@ -200,7 +200,8 @@ def append_kvcache_block_scaled(
     +-448; it grows, and the block's older codes are re-rounded, when a larger
     value arrives in a block that already holds tokens.
 
-    Returns the rotated ``query`` (in ``query_out`` when given), or None.
+    Returns the rotated ``query`` (in ``query_out`` when given, which may be
+    ``query`` itself), or None.
     """
     index = _cuda_index(key)
     _no_grad(key, value, query)

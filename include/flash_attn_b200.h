@@ -341,7 +341,7 @@ typedef struct fa_block_cache {
  */
 typedef struct fa_block_append_args {
   fa_tensor key, value;        /* [T,Hkv,D] f16/bf16/f32 */
-  fa_tensor query, query_out;  /* [T,Hq,D] f16/bf16/f32 or absent */
+  fa_tensor query, query_out;  /* [T,Hq,D] f16/bf16/f32 or absent; query_out may be query itself */
   fa_tensor cu_seqlens;        /* int32 [B+1] */
   fa_tensor seqlens;           /* int32 [B], lengths before the append */
   fa_tensor cos, sin;          /* f32 [positions, rot/2] or absent */

@@ -130,3 +130,20 @@ def test_prompt_chunks_over_any_scales(dtype, d):
     run_prefill(*args, mutate=mutate, sinks=True, window=70, first=20)
     run_prefill(*args, mutate=mutate, sinks=True, causal=False)
     run_prefill([130, 260], [20, 300], 32, 4, d, 16, 16, dtype, mutate=mutate, sinks=True)     # rows that see nothing
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("dtype,d,rot", [(torch.bfloat16, 128, 128), (torch.bfloat16, 128, 64), (torch.float16, 80, 20),
+                                         (torch.float32, 128, 128), (torch.bfloat16, 72, 40), (torch.float32, 63, 30)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_writes_query_out(dtype, d, rot, interleaved, in_place, monkeypatch):
+    """Queries rotated into a given tensor or in place, by the vector kernels and by the one for any layout."""
+    call = base.append_kvcache_block_scaled
+
+    def with_out(*args, query, **kw):
+        out = query if in_place else torch.full_like(query, float("nan"))
+        assert call(*args, query=query, query_out=out, **kw) is out
+        return out
+    monkeypatch.setattr(base, "append_kvcache_block_scaled", with_out)
+    for ns in ([9, 33, 1], [700, 41, 3]):                # one launch; queries in a launch of their own
+        base.run_append(ns, [5, 0, 31], 12, 2, d, 32, 16, dtype, rot=rot, interleaved=interleaved, seed=d)

@@ -446,6 +446,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_pick_kernel(const Ve
   if (!last) return;
   __threadfence();
   unsigned long long key = *reinterpret_cast<volatile unsigned long long*>(pl.best + b);
+  __syncthreads();  // every thread has read it before any raises it below
   if (!greedy && key == 0 && i < n) {
     // No residual anywhere: the target's own probabilities (this CTA alone; a
     // draft is rejected where q >= p throughout, which rounding alone allows).

@@ -147,3 +147,15 @@ def test_append_writes_query_out(dtype, d, rot, interleaved, in_place, monkeypat
     monkeypatch.setattr(base, "append_kvcache_block_scaled", with_out)
     for ns in ([9, 33, 1], [700, 41, 3]):                # one launch; queries in a launch of their own
         base.run_append(ns, [5, 0, 31], 12, 2, d, 32, 16, dtype, rot=rot, interleaved=interleaved, seed=d)
+
+
+@pytest.mark.parametrize("V", [1, 2, 33, 257, 1000, 4099, 151936])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_verify_without_residual(V, dtype):
+    """Rejected drafts whose q is above p everywhere: the token is drawn from p, whatever the vocabulary's size."""
+    def poke(logits, q, tokens, u, noise):
+        rows = [0, 1, 2, 4, 7, 8, 9, 10, 11]             # the drafts' rows of requests with 3, 1, 0 and 5 drafts
+        q.copy_(torch.softmax(logits[rows].float(), -1) * 1.125)
+        u.fill_(0.96875)
+    acc = base.run_verify([3, 1, 0, 5], V, dtype, seed=17 + V, poke=poke)
+    assert acc.tolist() == [0, 0, 0, 0]

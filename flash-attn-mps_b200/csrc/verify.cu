@@ -40,13 +40,20 @@ __device__ __forceinline__ void best_of(float& v, int& i, float w, int j) {
   if (w > v || (w == v && j < i)) { v = w; i = j; }
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
+
+// log2(e) / temperature. It multiplies differences to a row's maximum only: a
+// scaled score itself may need more than float32's bits (2^25 at a temperature
+// of 1e-6). Bounded, so that 0 and -inf stay what they are at any temperature.
+__device__ __forceinline__ float per_temperature(float temp) { return fminf(fmaxf(kLog2e / temp, 1e-30f), 1e30f); }
+
 // One CTA per request, rows in turn: strided vocabularies and very many rows.
 __global__ void __launch_bounds__(1024) verify_kernel(const VerifyArgs a) {
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int begin = a.cu[b * a.cu0], n = min(max(a.cu[(b + 1) * a.cu0] - begin, 0), a.K);
   const float temp = a.temp ? a.temp[b * a.te0] : 1.f;
   const bool greedy = !(temp > 0.f);
-  const float inv = greedy ? 1.f : 1.f / temp;
+  const float k = per_temperature(greedy ? 1.f : temp);
   __shared__ float sv[32], ss[32], sv2[32];
   __shared__ int si[32], si2[32];
   float mx = -INFINITY, sum = 0.f;
@@ -55,7 +62,7 @@ __global__ void __launch_bounds__(1024) verify_kernel(const VerifyArgs a) {
     const int64_t row = (int64_t)(begin + b + i) * a.xs0;
     float m = -INFINITY;
     int at = 0x7fffffff;
-    for (int v = tid; v < a.V; v += 1024) best_of(m, at, load_float(a.x, a.xt, row + v * a.xs1) * inv, v);
+    for (int v = tid; v < a.V; v += 1024) best_of(m, at, load_float(a.x, a.xt, row + v * a.xs1), v);
     for (int o = 16; o; o >>= 1) {
       const float w = __shfl_xor_sync(~0u, m, o);
       const int j = __shfl_xor_sync(~0u, at, o);
@@ -68,7 +75,7 @@ __global__ void __launch_bounds__(1024) verify_kernel(const VerifyArgs a) {
     if (hot >= a.V) hot = 0;
     float s = 0.f;
     if (!greedy)
-      for (int v = tid; v < a.V; v += 1024) s += expf(load_float(a.x, a.xt, row + v * a.xs1) * inv - mx);
+      for (int v = tid; v < a.V; v += 1024) s += fast_exp2((load_float(a.x, a.xt, row + v * a.xs1) - mx) * k);
     s = warp_sum(s);
     if (lane == 0) ss[warp] = s;
     __syncthreads();
@@ -78,17 +85,18 @@ __global__ void __launch_bounds__(1024) verify_kernel(const VerifyArgs a) {
     if (i >= n) break;
     const int64_t tok = load_index(a.tok, a.tt, (int64_t)(begin + i) * a.tk0);
     float p = 0.f;
-    if (tok >= 0 && tok < a.V) p = greedy ? (tok == hot ? 1.f : 0.f) : expf(load_float(a.x, a.xt, row + tok * a.xs1) * inv - mx) / sum;
+    if (tok >= 0 && tok < a.V) p = greedy ? (tok == hot ? 1.f : 0.f) : fast_exp2((load_float(a.x, a.xt, row + tok * a.xs1) - mx) * k) / sum;
     const float q = a.dp ? (tok >= 0 && tok < a.V ? load_float(a.dp, a.dt, (int64_t)(begin + i) * a.dp0 + tok * a.dp1) : 0.f) : 1.f;
     if (!(a.u[(int64_t)(begin + i) * a.u0] * q < p)) break;
   }
   // Row i: the first rejected draft's (i < n) or the one behind the last.
   const int64_t row = (int64_t)(begin + b + i) * a.xs0;
   const int64_t drafted = i < n && !a.dp ? load_index(a.tok, a.tt, (int64_t)(begin + i) * a.tk0) : -1;
+  const float is = 1.f / sum;
   float r = 0.f, f = 0.f;
   int ri = 0x7fffffff, fi = 0x7fffffff;
   for (int v = tid; v < a.V; v += 1024) {
-    const float p = greedy ? (v == hot ? 1.f : 0.f) : expf(load_float(a.x, a.xt, row + v * a.xs1) * inv - mx) / sum;
+    const float p = greedy ? (v == hot ? 1.f : 0.f) : fast_exp2((load_float(a.x, a.xt, row + v * a.xs1) - mx) * k) * is;
     float q = 0.f;
     if (i < n) q = a.dp ? load_float(a.dp, a.dt, (int64_t)(begin + i) * a.dp0 + v * a.dp1) : (v == drafted ? 1.f : 0.f);
     const float e = a.noise[(int64_t)b * a.no0 + v * a.no1];
@@ -114,7 +122,6 @@ __global__ void __launch_bounds__(1024) verify_kernel(const VerifyArgs a) {
   }
 }
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyCtas = 8;  // per SM that a pass is cut into (4 and 16 measured alike or slower)
 
@@ -123,7 +130,7 @@ struct VerifyPlan {
   int32_t rows, chunks, span;          // statistics: chunks of a row, their elements
   int32_t pick_chunks, pick_span;      // second pass, per request
   int32_t x_vec, y_vec;                // 16-byte vectors: logits; logits, draft rows and noise together
-  float4* stats;                       // [rows][chunks] {maximum * k, sum of 2^(x k - that), first maximum, -}
+  float4* stats;                       // [rows][chunks] {maximum, sum of 2^((x - it) k), first maximum, -}
   unsigned long long* best;            // [B] largest w / noise as (value bits, ~index)
   int32_t* done;                       // [B] CTAs of the second pass that are through
 };
@@ -151,9 +158,10 @@ struct Vec {
   static __device__ __forceinline__ float one(const void* p, int64_t off) { return load_float(p, DT, off); }
 };
 
-// Running maximum and sum of 2^(y - maximum) over values y (in log2 units).
+// Running maximum and sum of 2^((y - maximum) k) over values y.
 struct Running {
-  float m = -INFINITY, s = 0.f;
+  float k, m = -INFINITY, s = 0.f;
+  __device__ __forceinline__ explicit Running(float k) : k(k) {}
   template <int N>
   __device__ __forceinline__ void add(const float (&y)[N]) {
     float t[4];
@@ -163,15 +171,15 @@ struct Running {
     for (int i = 4; i < N; ++i) t[i & 3] = fmaxf(t[i & 3], y[i]);
     const float n = fmaxf(m, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
     const float c = n == -INFINITY ? 0.f : n;
-    float a[4] = {s * fast_exp2(m - c), 0.f, 0.f, 0.f};  // m = -inf: 0
+    float a[4] = {s * fast_exp2((m - c) * k), 0.f, 0.f, 0.f};  // m = -inf: 0
     m = n;
 #pragma unroll
-    for (int i = 0; i < N; ++i) a[i & 3] += fast_exp2(y[i] - c);
+    for (int i = 0; i < N; ++i) a[i & 3] += fast_exp2((y[i] - c) * k);
     s = (a[0] + a[1]) + (a[2] + a[3]);
   }
   __device__ __forceinline__ void join(float m2, float s2) {
     const float t = fmaxf(m, m2), c = t == -INFINITY ? 0.f : t;
-    s = s * fast_exp2(m - c) + s2 * fast_exp2(m2 - c);
+    s = s * fast_exp2((m - c) * k) + s2 * fast_exp2((m2 - c) * k);
     m = t;
   }
 };
@@ -226,8 +234,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_stats_kernel(const Veri
   load(tid, x);  // on its way while the row's request is looked up
   const float temp = a.temp ? __ldg(a.temp + (int64_t)request_of(a, r, lane) * a.te0) : 1.f;
   const bool greedy = !(temp > 0.f);
-  const float k = (greedy ? 1.f : 1.f / temp) * kLog2e;
-  Running run;
+  Running run(per_temperature(greedy ? 1.f : temp));
   float top = -INFINITY;
   int at = 0x7fffffff;
   for (int i0 = tid; i0 < nvec; i0 += kU * kVerifyThreads) {
@@ -237,8 +244,6 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_stats_kernel(const Veri
 #pragma unroll
         for (int h = 0; h < N; ++h) rising(top, at, x[q * N + h], b0 + (i0 + q * kVerifyThreads) * N + h);
     } else {
-#pragma unroll
-      for (int h = 0; h < kU * N; ++h) x[h] *= k;
       run.add(x);
     }
     if (i0 + kU * kVerifyThreads < nvec) load(i0 + kU * kVerifyThreads, x);
@@ -246,7 +251,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_stats_kernel(const Veri
   auto use_one = [&](int v) {
     const float y = V::one(a.x, row + v);
     if (greedy) best_of(top, at, y, v);
-    else run.join(y * k, y == -INFINITY ? 0.f : 1.f);
+    else run.join(y, y == -INFINITY ? 0.f : 1.f);
   };
   if (pl.x_vec && tid < head) use_one(v0 + tid);
   for (int v = (pl.x_vec ? b0 + nvec * N : v0) + tid; v < v1; v += kVerifyThreads) use_one(v);
@@ -317,7 +322,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_pick_kernel(const Ve
   const int begin = a.cu[b * a.cu0], n = min(max(a.cu[(b + 1) * a.cu0] - begin, 0), a.K);
   const float temp = a.temp ? a.temp[b * a.te0] : 1.f;
   const bool greedy = !(temp > 0.f);
-  const float k = (greedy ? 1.f : 1.f / temp) * kLog2e;
+  const float k = per_temperature(greedy ? 1.f : temp);
   // What does not depend on the statistics is read while they are computed:
   // a warp's draft and this thread's first noise.
   const int v0 = chunk * pl.pick_span, v1 = min(a.V, v0 + pl.pick_span);
@@ -349,7 +354,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_pick_kernel(const Ve
   // A row's maximum, sum and first maximum, by one warp.
   auto row_stats = [&](int i, float& m, float& s, int& hot) {
     const float4* st = pl.stats + (int64_t)(begin + b + i) * pl.chunks;
-    Running run;
+    Running run(k);
     float top = -INFINITY;
     int at = 0x7fffffff;
     for (int c = lane; c < pl.chunks; c += 32) {
@@ -375,7 +380,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_pick_kernel(const Ve
     if (i == n) break;
     const Draft d = i == warp ? mine : draft_of(i);
     float p = 0.f;
-    if (d.in) p = greedy ? (d.tok == hot ? 1.f : 0.f) : fast_exp2(d.x * k - m) / s;
+    if (d.in) p = greedy ? (d.tok == hot ? 1.f : 0.f) : fast_exp2((d.x - m) * k) / s;
     if (lane == 0 && !(d.u * d.q < p)) atomicMin(&first_no, i);
   }
   __syncthreads();
@@ -400,7 +405,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_pick_kernel(const Ve
     const int64_t drafted = i < n && !a.dp ? load_index(a.tok, a.tt, (int64_t)(begin + i) * a.tk0) : -1;
     const float is = 1.f / s;
     auto use = [&](float x, float q, float e, int v) {
-      const float w = fast_exp2(x * k - m) * is - (v == drafted ? 1.f : q);
+      const float w = fast_exp2((x - m) * k) * is - (v == drafted ? 1.f : q);
       float ie;
       asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(ie) : "f"(e));
       if (w > 0.f) rising(r, ri, w * ie, v);
@@ -454,7 +459,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_pick_kernel(const Ve
     r = -1.f;
     ri = 0x7fffffff;
     for (int v = tid; v < a.V; v += kVerifyThreads) {
-      const float p = fast_exp2(V::one(a.x, row + v) * k - m) / s;
+      const float p = fast_exp2((V::one(a.x, row + v) - m) * k) / s;
       if (p > 0.f) rising(r, ri, p / a.noise[nrow + v], v);
     }
 #pragma unroll

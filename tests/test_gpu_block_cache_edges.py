@@ -159,3 +159,24 @@ def test_verify_without_residual(V, dtype):
         u.fill_(0.96875)
     acc = base.run_verify([3, 1, 0, 5], V, dtype, seed=17 + V, poke=poke)
     assert acc.tolist() == [0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("strided", [False, True])
+def test_verify_low_temperatures(dtype, strided, monkeypatch):
+    """Scores of up to 2^26 at a temperature: only differences to the row's maximum may be scaled by it."""
+    call = base.verify_draft_tokens
+    if strided:                                          # vocabulary not contiguous
+        monkeypatch.setattr(base, "verify_draft_tokens",
+                            lambda logits, *args, **kw: call(logits.t().contiguous().t(), *args, **kw))
+
+    def likeliest(logits, q, tokens, u, noise):
+        rows = [b + i for b in range(4) for i in range(3 * b, 3 * b + 3)]
+        tokens.copy_(logits[rows].float().argmax(-1))
+        u.fill_(0.75)
+    temps = [1e-6, 1e-5, 1e-4, 1e-3]
+    for seed in range(4):
+        base.run_verify([3, 3, 3, 3], 1009, dtype, one_hot=True, temps=temps, seed=seed, poke=likeliest)
+        base.run_verify([3, 3, 3, 3], 1009, dtype, temps=temps, seed=seed, poke=likeliest)
+        base.run_verify([3, 3, 3, 3], 1009, dtype, temps=[1e-2, 3e-2, 1e-1, 30.0], seed=seed)
+    base.run_verify([3, 3, 3, 3], 1009, dtype, one_hot=True, temps=[1e-38, 1e-44, 1e30, 1.0], seed=7, poke=likeliest)

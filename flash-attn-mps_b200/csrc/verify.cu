@@ -47,6 +47,38 @@ constexpr float kLog2e = 1.4426950408889634f;
 // of 1e-6). Bounded, so that 0 and -inf stay what they are at any temperature.
 __device__ __forceinline__ float per_temperature(float temp) { return fminf(fmaxf(kLog2e / temp, 1e-30f), 1e30f); }
 
+// Order of w / e at token v as an integer: the larger quotient, then the lower
+// token; 0 without one (w not positive, e negative or NaN). float32 holds neither
+// 1 / 2^-149 nor 2^-30 / 2^127: the mantissas' quotient is rounded to float32 and
+// takes the exponents' difference beside it (its 23 bits and 9 of exponent fit 32).
+__device__ __forceinline__ unsigned long long quotient_key(float w, float e, int v) {
+  if (!(w > 0.f && e >= 0.f)) return 0;
+  uint32_t key = 1;                              // e infinite
+  if (e == 0.f || w == INFINITY) {
+    key = 0xffffffffu;
+  } else if (e < INFINITY) {
+    int shift = 256;                             // of the quotient's exponent field
+    if (w < 0x1p-126f) { w *= 0x1p24f; shift -= 24; }
+    if (e < 0x1p-126f) { e *= 0x1p24f; shift += 24; }
+    const uint32_t wb = __float_as_uint(w), eb = __float_as_uint(e);
+    const float q = __fdiv_rn(__uint_as_float((wb & 0x7fffffu) | 0x3f800000u), __uint_as_float((eb & 0x7fffffu) | 0x3f800000u));
+    shift += (int)(wb >> 23) - (int)(eb >> 23);  // |difference| < 256 + 24
+    const int64_t k = (int64_t)__float_as_uint(q) + ((int64_t)(shift - 127) << 23);
+    key = (uint32_t)min(max(k, (int64_t)1), (int64_t)0xfffffffe);
+  }
+  return (unsigned long long)key << 32 | (0xffffffffu - (uint32_t)v);
+}
+// The same of a quotient that float32 holds.
+__device__ __forceinline__ unsigned long long quotient_key(float y, int v) {
+  return (unsigned long long)(__float_as_uint(y) + (129u << 23)) << 32 | (0xffffffffu - (uint32_t)v);
+}
+__device__ __forceinline__ int token_of(unsigned long long key) { return (int)(0xffffffffu - (uint32_t)key); }
+__device__ __forceinline__ unsigned long long warp_max_key(unsigned long long k) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) k = max(k, __shfl_xor_sync(~0u, k, o));
+  return k;
+}
+
 // One CTA per request, rows in turn: strided vocabularies and very many rows.
 __global__ void __launch_bounds__(1024) verify_kernel(const VerifyArgs a) {
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -54,8 +86,9 @@ __global__ void __launch_bounds__(1024) verify_kernel(const VerifyArgs a) {
   const float temp = a.temp ? a.temp[b * a.te0] : 1.f;
   const bool greedy = !(temp > 0.f);
   const float k = per_temperature(greedy ? 1.f : temp);
-  __shared__ float sv[32], ss[32], sv2[32];
-  __shared__ int si[32], si2[32];
+  __shared__ float sv[32], ss[32];
+  __shared__ int si[32];
+  __shared__ unsigned long long sr[32], sf[32];
   float mx = -INFINITY, sum = 0.f;
   int hot = 0, i = 0;
   for (;; ++i) {
@@ -93,29 +126,22 @@ __global__ void __launch_bounds__(1024) verify_kernel(const VerifyArgs a) {
   const int64_t row = (int64_t)(begin + b + i) * a.xs0;
   const int64_t drafted = i < n && !a.dp ? load_index(a.tok, a.tt, (int64_t)(begin + i) * a.tk0) : -1;
   const float is = 1.f / sum;
-  float r = 0.f, f = 0.f;
-  int ri = 0x7fffffff, fi = 0x7fffffff;
+  unsigned long long r = 0, f = 0;  // best of the residual, of p
   for (int v = tid; v < a.V; v += 1024) {
     const float p = greedy ? (v == hot ? 1.f : 0.f) : fast_exp2((load_float(a.x, a.xt, row + v * a.xs1) - mx) * k) * is;
     float q = 0.f;
     if (i < n) q = a.dp ? load_float(a.dp, a.dt, (int64_t)(begin + i) * a.dp0 + v * a.dp1) : (v == drafted ? 1.f : 0.f);
     const float e = a.noise[(int64_t)b * a.no0 + v * a.no1];
-    if (p > 0.f) best_of(f, fi, p / e, v);
-    if (p - q > 0.f) best_of(r, ri, (p - q) / e, v);
+    f = max(f, quotient_key(p, e, v));
+    r = max(r, quotient_key(p - q, e, v));
   }
-  for (int o = 16; o; o >>= 1) {
-    float w = __shfl_xor_sync(~0u, r, o);
-    int j = __shfl_xor_sync(~0u, ri, o);
-    best_of(r, ri, w, j);
-    w = __shfl_xor_sync(~0u, f, o);
-    j = __shfl_xor_sync(~0u, fi, o);
-    best_of(f, fi, w, j);
-  }
-  if (lane == 0) { sv[warp] = r; si[warp] = ri; sv2[warp] = f; si2[warp] = fi; }
+  r = warp_max_key(r);
+  f = warp_max_key(f);
+  if (lane == 0) { sr[warp] = r; sf[warp] = f; }
   __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < 32; ++w) { best_of(r, ri, sv[w], si[w]); best_of(f, fi, sv2[w], si2[w]); }
-    const int got = ri < a.V ? ri : fi < a.V ? fi : 0;
+    for (int w = 1; w < 32; ++w) { r = max(r, sr[w]); f = max(f, sf[w]); }
+    const int got = r ? token_of(r) : f ? token_of(f) : 0;
     for (int k = 0; k <= a.K; ++k)
       a.out[b * a.o0 + k * a.o1] = k < i ? load_index(a.tok, a.tt, (int64_t)(begin + k) * a.tk0) : k == i ? got : -1;
     a.acc[b * a.a0] = i;
@@ -131,7 +157,7 @@ struct VerifyPlan {
   int32_t pick_chunks, pick_span;      // second pass, per request
   int32_t x_vec, y_vec;                // 16-byte vectors: logits; logits, draft rows and noise together
   float4* stats;                       // [rows][chunks] {maximum, sum of 2^((x - it) k), first maximum, -}
-  unsigned long long* best;            // [B] largest w / noise as (value bits, ~index)
+  unsigned long long* best;            // [B] largest w / noise (quotient_key)
   int32_t* done;                       // [B] CTAs of the second pass that are through
 };
 
@@ -274,11 +300,6 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_stats_kernel(const Veri
   }
 }
 
-// Key of a positive value at an index: larger values first, then lower indices.
-__device__ __forceinline__ unsigned long long key_of(float v, int i) {
-  return (unsigned long long)__float_as_uint(v) << 32 | (0xffffffffu - (uint32_t)i);
-}
-
 constexpr int kPick = 1;    // vectors of a thread in flight (2 need the registers of a CTA per SM: 50 us against 46)
 constexpr int kRows = 64;   // rows of a request whose numbers stay in shared memory
 
@@ -397,19 +418,21 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_pick_kernel(const Ve
   const float4 st = rows[i < kRows ? i : 0];
   const int shot = __float_as_int(st.z);
   const float m = st.x, s = st.y;
-  float r = -1.f;
-  int ri = 0x7fffffff;
+  unsigned long long best = 0;
   if (!greedy) {
     const int64_t row = (int64_t)(begin + b + i) * a.xs0, qrow = (int64_t)(begin + i) * a.dp0;
     const bool with_q = i < n && a.dp;
     const int64_t drafted = i < n && !a.dp ? load_index(a.tok, a.tt, (int64_t)(begin + i) * a.tk0) : -1;
     const float is = 1.f / s;
-    auto use = [&](float x, float q, float e, int v) {
-      const float w = fast_exp2((x - m) * k) * is - (v == drafted ? 1.f : q);
-      float ie;
-      asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(ie) : "f"(e));
-      if (w > 0.f) rising(r, ri, w * ie, v);
+    auto weight = [&](float x, float q, int v) { return fast_exp2((x - m) * k) * is - (v == drafted ? 1.f : q); };
+    auto divide = [&](int v) {
+      const float w = weight(V::one(a.x, row + v), with_q ? load_float(a.dp, a.dt, qrow + v) : 0.f, v);
+      best = max(best, quotient_key(w, a.noise[nrow + v], v));
     };
+    // w / e by an approximate reciprocal, good to 2^-22 as w itself; by a division
+    // where that leaves float32's range.
+    float r = -1.f;
+    int ri = 0x7fffffff;
     if (pl.y_vec) {
       for (int w0 = v0; w0 < v1; w0 += kPick * kVerifyThreads * N) {
         float x[kPick][N], y[kPick][N];
@@ -424,24 +447,32 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_pick_kernel(const Ve
         for (int q = 0; q < kPick; ++q) {
           const int v = w0 + (tid + q * kVerifyThreads) * N;
           if (v < v1) {
+            bool odd = false;
 #pragma unroll
-            for (int h = 0; h < N; ++h) use(x[q][h], y[q][h], e0[q][h], v + h);
+            for (int h = 0; h < N; ++h) {
+              const float w = weight(x[q][h], y[q][h], v + h);
+              float ie;
+              asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(ie) : "f"(e0[q][h]));
+              const float z = w * ie;
+              if (z >= 0x1p-126f && z <= 0x1p100f) rising(r, ri, z, v + h);
+              else odd |= w > 0.f;
+            }
+            if (odd) {
+#pragma unroll 1
+              for (int h = 0; h < N; ++h) divide(v + h);
+            }
           }
         }
       }
+      if (ri < a.V) best = max(best, quotient_key(r, ri));
     } else {
 #pragma unroll 4
-      for (int v = v0 + tid; v < v1; v += kVerifyThreads)
-        use(V::one(a.x, row + v), with_q ? load_float(a.dp, a.dt, qrow + v) : 0.f, a.noise[nrow + v], v);
+      for (int v = v0 + tid; v < v1; v += kVerifyThreads) divide(v);
     }
   }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const float w = __shfl_xor_sync(~0u, r, o);
-    best_of(r, ri, w, __shfl_xor_sync(~0u, ri, o));
-  }
+  best = warp_max_key(best);
   if (lane == 0) {
-    if (ri < a.V) atomicMax(pl.best + b, key_of(r, ri));
+    if (best) atomicMax(pl.best + b, best);
     __threadfence();
   }
   __syncthreads();
@@ -456,23 +487,19 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_pick_kernel(const Ve
     // No residual anywhere: the target's own probabilities (this CTA alone; a
     // draft is rejected where q >= p throughout, which rounding alone allows).
     const int64_t row = (int64_t)(begin + b + i) * a.xs0;
-    r = -1.f;
-    ri = 0x7fffffff;
+    const float is = 1.f / s;
+    best = 0;
     for (int v = tid; v < a.V; v += kVerifyThreads) {
-      const float p = fast_exp2((V::one(a.x, row + v) - m) * k) / s;
-      if (p > 0.f) rising(r, ri, p / a.noise[nrow + v], v);
+      const float p = fast_exp2((V::one(a.x, row + v) - m) * k) * is;
+      best = max(best, quotient_key(p, a.noise[nrow + v], v));
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float w = __shfl_xor_sync(~0u, r, o);
-      best_of(r, ri, w, __shfl_xor_sync(~0u, ri, o));
-    }
-    if (lane == 0 && ri < a.V) atomicMax(pl.best + b, key_of(r, ri));
+    best = warp_max_key(best);
+    if (lane == 0 && best) atomicMax(pl.best + b, best);
     __threadfence();
     __syncthreads();
     key = *reinterpret_cast<volatile unsigned long long*>(pl.best + b);
   }
-  const int got = greedy ? shot : key ? (int)(0xffffffffu - (uint32_t)key) : 0;
+  const int got = greedy ? shot : key ? token_of(key) : 0;
   for (int j = tid; j <= a.K; j += kVerifyThreads)
     a.out[b * a.o0 + j * a.o1] = j < i ? load_index(a.tok, a.tt, (int64_t)(begin + j) * a.tk0) : j == i ? got : -1;
   if (tid == 0) a.acc[b * a.a0] = i;

@@ -180,3 +180,24 @@ def test_verify_low_temperatures(dtype, strided, monkeypatch):
         base.run_verify([3, 3, 3, 3], 1009, dtype, temps=temps, seed=seed, poke=likeliest)
         base.run_verify([3, 3, 3, 3], 1009, dtype, temps=[1e-2, 3e-2, 1e-1, 30.0], seed=seed)
     base.run_verify([3, 3, 3, 3], 1009, dtype, one_hot=True, temps=[1e-38, 1e-44, 1e30, 1.0], seed=7, poke=likeliest)
+
+
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("size", [1e-44, 1e-38, 1e-30, 1.0, 1e30, 2.0 ** 126])
+def test_verify_noise_of_any_size(size, strided, monkeypatch):
+    """Quotients by the smallest and largest noise that float32 holds, with and without a contiguous vocabulary."""
+    call = base.verify_draft_tokens
+    if strided:
+        monkeypatch.setattr(base, "verify_draft_tokens",
+                            lambda logits, *args, **kw: call(logits.t().contiguous().t(), *args, **kw))
+
+    def poke(logits, q, tokens, u, noise):
+        g = torch.Generator().manual_seed(5)
+        at = torch.randint(1, 3, noise.shape, generator=g)
+        noise.copy_(size * at.double())
+        logits.copy_(-40.0 - torch.rand(logits.shape, generator=g))
+        logits[:, 700] = 1.0                             # probabilities of 0.6 and 0.4 decide
+        logits[:, 300] = 0.6
+        noise[:, 300] = size * 2
+    for one_hot in (False, True):
+        base.run_verify([2, 0, 3], 1024, torch.float32, one_hot=one_hot, seed=3, poke=poke)

@@ -223,11 +223,11 @@ def append_kvcache_block_scaled(
         rotary_sin = rotary_sin.float()
     if cache_seqlens.ndim != 1:
         raise ValueError("cache_seqlens must be int32 [batch]")
-    _, view = _APPEND.pack(
-        (_packed(key, "key"), _packed(value, "value"), None if query is None else _packed(query, "query"),
-         None if query is None else _packed(query_out, "query_out"), cu, cache_seqlens, rotary_cos, rotary_sin, positions,
-         rotary_axes, k_cache, v_cache, k_scale, v_scale, block_table),
-        (cache_seqlens.shape[0], longest, bool(rotary_interleaved)), index)
+    # Held until the launch: a head-major tensor's packed form is a copy, whose memory another thread could be given.
+    tensors = (_packed(key, "key"), _packed(value, "value"), None if query is None else _packed(query, "query"),
+               None if query is None else _packed(query_out, "query_out"), cu, cache_seqlens, rotary_cos, rotary_sin,
+               positions, rotary_axes, k_cache, v_cache, k_scale, v_scale, block_table)
+    _, view = _APPEND.pack(tensors, (cache_seqlens.shape[0], longest, bool(rotary_interleaved)), index)
     _call(_capi.library().fa_append_block_scaled, view, index)
     return query_out if query is not None else None
 

@@ -1,6 +1,7 @@
 """Block-scaled cache operators on the CPU: host checks, the axis map, and the host oracle against itself."""
 
 import ctypes
+import weakref
 
 import numpy as np
 import pytest
@@ -103,3 +104,26 @@ def test_oracle_verification_samples_the_target():
     got = np.bincount(out[:, 0], minlength=V) / n
     assert np.abs(got - p).max() < 5 * np.sqrt(0.25 / n)
     assert 0 < accepted.mean() < 1
+
+
+def test_packed_copies_live_until_the_launch(monkeypatch):
+    """Head-major keys, values and queries are copied into packed rows; the copies must not be freed before the launch."""
+    made, alive = [], []
+    packed = block_cache._packed
+
+    def watched(x, name):
+        out = packed(x, name)
+        made.append(weakref.ref(out))
+        return out
+
+    def launch(fn, view, index):
+        alive.extend(ref() is not None for ref in made)
+    monkeypatch.setattr(block_cache, "_packed", watched)
+    monkeypatch.setattr(block_cache, "_cuda_index", lambda x: 0)
+    monkeypatch.setattr(block_cache, "_call", launch)
+    monkeypatch.setattr(block_cache._Arguments, "pack", lambda self, tensors, scalars, index: (None, None))
+    x = torch.randn(2, 3, 5, 64).transpose(1, 2)             # [batch, new, heads, dim], heads outermost in memory
+    cache, scale = torch.zeros(2, 16, 3, 64).to(torch.float8_e4m3fn), torch.ones(2, 1, 3)
+    append_kvcache_block_scaled(x, x, cache, cache, scale, scale, torch.zeros(2, dtype=torch.int32),
+                                torch.zeros(2, 2, dtype=torch.int32), query=x)
+    assert len(made) == 4 and all(alive) and len(alive) == 4

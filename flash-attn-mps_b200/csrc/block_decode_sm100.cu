@@ -514,8 +514,8 @@ __global__ void __launch_bounds__(Shape<NP, C, DH>::kThreads, Shape<NP, C, DH>::
       rec[(u % kUnitRing) * R_WORDS + R_B] = -1;
       mbar_arrive(bar(Sh::B_UF + u % kUnitRing));
     }
-    // Every issued copy lands before the CTA leaves.
-    for (int i = max(0, 2 * gt - NSLOT); ok && i < 2 * gt; ++i)
+    // Every issued copy lands before the CTA leaves, after a time-out too.
+    for (int i = max(0, 2 * gt - NSLOT); i < 2 * gt; ++i)
       if (i % 2 == 0) wait_all(bar(Sh::B_FULL + i % NSLOT), (i / NSLOT) & 1);
   } else if (warp == 4 * WG + 3) {
     // ----------------------------------------------------------- V page gathers
@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(Shape<NP, C, DH>::kThreads, Shape<NP, C, DH>::
         pg0 = pg1; pg1 = pg2;
       }
     }
-    for (int i = max(0, 2 * gt - NSLOT); ok && i < 2 * gt; ++i)
+    for (int i = max(0, 2 * gt - NSLOT); i < 2 * gt; ++i)
       if (i % 2 == 1) wait_all(bar(Sh::B_FULL + i % NSLOT), (i / NSLOT) & 1);
   } else if (warp == 4 * WG + 1) {
     // --------------------------------------------------------------------- MMA

@@ -367,10 +367,14 @@ int fill(const fa_block_attention_args* g, BlockAttn* p) {
   p->used = (const int32_t*)g->seqlens.ptr; p->u0 = g->seqlens.stride[0];
   if (present(g->s_aux)) { p->sinks = g->s_aux.ptr; p->sink_t = g->s_aux.dtype; p->si0 = g->s_aux.stride[0]; }
   p->T = (int32_t)g->q.shape[0]; p->B = g->batch; p->HQ = (int32_t)g->q.shape[1];
-  p->max_q = g->max_seqlen_q; p->max_k = g->max_seqlen_k;
+  // Bounds of any size up to 2^31 - 1 may be given: beyond the rows, the block
+  // table and 2^30 keys they mean no more than these, and their sums and
+  // differences stay within 32 bits.
+  const int32_t capacity = std::min(p->c.bt_cols * p->c.page, 1 << 30);
+  p->max_q = std::min(g->max_seqlen_q, p->T); p->max_k = std::min(g->max_seqlen_k, capacity);
   p->causal = g->causal != 0;
-  p->win = g->window_left < 0 ? -1 : g->window_left;
-  p->first = p->win >= 0 ? g->first_tokens : 0;
+  p->win = g->window_left < 0 || g->window_left >= capacity ? -1 : g->window_left;
+  p->first = p->win >= 0 ? std::min(g->first_tokens, capacity) : 0;
   p->splits = g->num_splits;
   p->scale = g->softmax_scale;
   return FA_OK;

@@ -201,3 +201,26 @@ def test_verify_noise_of_any_size(size, strided, monkeypatch):
         noise[:, 300] = size * 2
     for one_hot in (False, True):
         base.run_verify([2, 0, 3], 1024, torch.float32, one_hot=one_hot, seed=3, poke=poke)
+
+
+BIG = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("ns,lens", [([1, 1], [300, 129]), ([4, 2], [300, 129]), ([5, 3], [3, 0]), ([130, 260], [500, 300])])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_bounds_of_any_size(dtype, ns, lens):
+    """Windows, first tokens and length bounds up to the largest 32-bit number."""
+    heads = (32, 2) if max(ns) > 100 else (8, 2)
+    if dtype == torch.float32 and max(ns) > 100:
+        heads, ns = (2, 1), [40, 60]
+    run_attention(ns, lens, *heads, 128, 16, 16, dtype, window=20, first=BIG)
+    run_attention(ns, lens, *heads, 128, 16, 16, dtype, window=BIG, first=3)
+    run_attention(ns, lens, *heads, 128, 16, 16, dtype, window=BIG - 1, first=BIG, max_k=BIG)
+    g = torch.Generator().manual_seed(1)
+    kc, vc, ks, vs, table = base.make_cache(g, lens, 16, 16, heads[1], 128)
+    q = torch.randn(sum(ns), heads[0], 128, generator=g).to(dtype).cuda()
+    used, cu = torch.tensor(lens, dtype=torch.int32).cuda(), base.offsets(ns)
+    call = base.flash_attn_with_block_scaled_kvcache
+    want = call(q, kc, vc, ks, vs, used, table, cu_seqlens_q=cu, max_seqlen_q=sum(ns), max_seqlen_k=table.shape[1] * 16)
+    got = call(q, kc, vc, ks, vs, used, table, cu_seqlens_q=cu, max_seqlen_q=BIG, max_seqlen_k=BIG)
+    assert torch.equal(got, want)

@@ -595,6 +595,8 @@ extern "C" int fa_append_block_scaled(const fa_block_append_args* g, void* strea
                       g->positions.shape[g->positions.ndim - 1] == T,
                   "positions must be int32 [tokens] or [axes, tokens]");
     a.pos = (const int32_t*)g->positions.ptr;
+    FAB_CHECK_ARG(g->positions.ndim == 1 || (g->positions.shape[0] >= 1 && g->positions.shape[0] < (1 << 16)),
+                  "positions must have at least one axis");
     a.n_axes = g->positions.ndim == 2 ? (int32_t)g->positions.shape[0] : 1;
     a.ps0 = g->positions.ndim == 2 ? g->positions.stride[0] : 0;
     a.ps1 = g->positions.stride[g->positions.ndim - 1];

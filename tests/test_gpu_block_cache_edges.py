@@ -224,3 +224,14 @@ def test_bounds_of_any_size(dtype, ns, lens):
     want = call(q, kc, vc, ks, vs, used, table, cu_seqlens_q=cu, max_seqlen_q=sum(ns), max_seqlen_k=table.shape[1] * 16)
     got = call(q, kc, vc, ks, vs, used, table, cu_seqlens_q=cu, max_seqlen_q=BIG, max_seqlen_k=BIG)
     assert torch.equal(got, want)
+
+
+def test_append_refuses_positions_without_axes():
+    g = torch.Generator().manual_seed(1)
+    kc, vc, ks, vs, table = base.make_cache(g, [64, 64], 16, 16, 2, 128)
+    k = torch.randn(2, 1, 2, 128, generator=g).to(torch.bfloat16).cuda()
+    used = torch.tensor([3, 9], dtype=torch.int32).cuda()
+    cos = torch.ones(64, 64).cuda()
+    with pytest.raises(ValueError, match="axis"):
+        base.append_kvcache_block_scaled(k, k, kc, vc, ks, vs, used, table, rotary_cos=cos, rotary_sin=cos,
+                                         positions=torch.zeros(0, 2, dtype=torch.int32).cuda())

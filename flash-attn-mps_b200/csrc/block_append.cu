@@ -54,6 +54,11 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a < INFINITY ? a : 0.f;  // infinities and NaN do not set a scale
 }
 
+// Whether a request's new tokens begin within its table row (what lies behind it is skipped).
+__device__ __forceinline__ bool starts_inside(const BlockCache& c, int start) {
+  return start >= 0 && start >> c.page_shift < c.bt_cols;
+}
+
 // cos/sin of pair i at a token row; positions are clamped to the tables.
 __device__ __forceinline__ int row_position(const AppendArgs& a, int axis, int64_t t, int abs_pos) {
   int p = abs_pos;
@@ -104,7 +109,7 @@ __global__ void __launch_bounds__(256) block_append_any_kernel(const AppendArgs 
   const int h = blockIdx.x % c.HK, u = blockIdx.x / c.HK;
   const int blk = (start >> c.block_shift) + u;
   const int base = blk << c.block_shift;
-  if (start < 0 || base >= start + n) return;
+  if (!starts_inside(c, start) || base >= start + n) return;
   const int pg = block_page(c, b, base);
   if (pg < 0) return;
   const int r0 = max(start - base, 0), r1 = min(start + n - base, c.block);
@@ -350,7 +355,7 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 8 ? 2 : 1) block_append_v
   // Unit: heads fastest, then K and V, then blocks: a CTA's warps write neighbouring rows.
   const int id = blockIdx.x * per_cta + in_cta, hs = id / c.HK, h = id - hs * c.HK, side = hs & 1, u = hs >> 1;
   const int base = ((start >> c.block_shift) + u) << c.block_shift;
-  bool live = in_cta < per_cta && u < a.units_per_req && n > 0 && start >= 0 && base < start + n;
+  bool live = in_cta < per_cta && u < a.units_per_req && n > 0 && starts_inside(c, start) && base < start + n;
   if (!__syncthreads_or(live)) return;
   const int r0 = max(start - base, 0), r1 = live ? min(start + n - base, c.block) : 0;
   const int tok0 = base & (c.page - 1);
@@ -564,7 +569,7 @@ extern "C" int fa_append_block_scaled(const fa_block_append_args* g, void* strea
                 "cu_seqlens must be int32 [batch + 1]");
   FAB_CHECK_ARG(present(g->seqlens) && g->seqlens.dtype == FA_I32 && g->seqlens.ndim == 1 && g->seqlens.shape[0] == g->batch,
                 "seqlens must be int32 [batch]");
-  a.B = g->batch; a.T = (int32_t)T; a.max_new = g->max_seqlen;
+  a.B = g->batch; a.T = (int32_t)T; a.max_new = std::min(g->max_seqlen, a.T);  // any upper bound may be given
   a.x[0] = g->key.ptr; a.x[1] = g->value.ptr; a.xt = g->key.dtype;
   const fa_tensor* xs[2] = {&g->key, &g->value};
   for (int i = 0; i < 2; ++i) { a.xs0[i] = xs[i]->stride[0]; a.xs1[i] = xs[i]->stride[1]; a.xs2[i] = xs[i]->stride[2]; }
@@ -607,11 +612,11 @@ extern "C" int fa_append_block_scaled(const fa_block_append_args* g, void* strea
     a.axes = (const int32_t*)g->rotary_axes.ptr; a.ax0 = g->rotary_axes.stride[0];
   }
   if (T == 0 || g->max_seqlen == 0) return FA_OK;
-  a.units_per_req = (g->max_seqlen + a.c.block - 2) / a.c.block + 1;
+  a.units_per_req = (int32_t)(((int64_t)a.max_new + a.c.block - 2) / a.c.block + 1);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (vector_rows(a)) {
     const int groups = a.c.D / 16, rows = kPasses * (32 / groups);
-    a.unit_warps = (std::min(a.c.block, g->max_seqlen) + rows - 1) / rows;
+    a.unit_warps = (std::min(a.c.block, a.max_new) + rows - 1) / rows;
     a.warps = a.unit_warps > 8 ? 16 : 8;
     const int per_cta = a.warps / a.unit_warps;
     const int64_t kv = ((int64_t)a.units_per_req * 2 * a.c.HK + per_cta - 1) / per_cta;  // CTAs of a request
@@ -643,6 +648,7 @@ extern "C" int fa_append_block_scaled(const fa_block_append_args* g, void* strea
     FAB_LAUNCH_CHECK("block-scaled append launch");
     return FA_OK;
   }
+  FAB_CHECK_ARG((int64_t)a.units_per_req * a.c.HK < (1LL << 31), "too many tokens for one append");
   const dim3 grid((unsigned)(a.units_per_req * a.c.HK), (unsigned)a.B, a.q ? 3u : 2u);
   block_append_any_kernel<<<grid, 256, 0, st>>>(a);
   note_launch();

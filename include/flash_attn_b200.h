@@ -348,7 +348,7 @@ typedef struct fa_block_append_args {
   fa_tensor positions;         /* int32 [T] or [axes,T], or absent */
   fa_tensor rotary_axes;       /* int32 [rot/2] or absent */
   fa_block_cache cache;
-  int32_t batch, max_seqlen;   /* max_seqlen: most new tokens of a request */
+  int32_t batch, max_seqlen;   /* max_seqlen: most new tokens of a request, or any upper bound */
   int32_t interleaved;
 } fa_block_append_args;
 

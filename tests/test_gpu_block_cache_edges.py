@@ -235,3 +235,21 @@ def test_append_refuses_positions_without_axes():
     with pytest.raises(ValueError, match="axis"):
         base.append_kvcache_block_scaled(k, k, kc, vc, ks, vs, used, table, rotary_cos=cos, rotary_sin=cos,
                                          positions=torch.zeros(0, 2, dtype=torch.int32).cuda())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_append_bounds_of_any_size(dtype, monkeypatch):
+    """Any upper bound of new tokens; requests whose length lies behind their table row append nothing."""
+    call = base.append_kvcache_block_scaled
+    monkeypatch.setattr(base, "append_kvcache_block_scaled", lambda *args, **kw: call(*args, **dict(kw, max_seqlen=BIG)))
+    base.run_append([1, 5, 0, 37], [0, 15, 3, 130], 6, 2, 128, 64, 32, dtype)
+    base.run_append([1, 1], [63, 64], 6, 2, 128, 64, 64, dtype)
+    g = torch.Generator().manual_seed(1)
+    kc, vc, ks, vs, table = base.make_cache(g, [64, 64, 64], 16, 16, 2, 128)
+    x = torch.randn(90, 2, 128, generator=g).to(dtype).cuda()
+    lens = [BIG - 20, table.shape[1] * 16, -5]
+    before = [base.np_of(t).copy() for t in (kc, vc, ks, vs)]
+    call(x, x, kc, vc, ks, vs, torch.tensor(lens, dtype=torch.int32).cuda(), table, cu_seqlens=base.offsets([15, 40, 35]),
+         max_seqlen=BIG)
+    for t, want in zip((kc, vc, ks, vs), before):
+        assert np.array_equal(base.np_of(t), want)

@@ -56,7 +56,10 @@ class _Arguments:
             for i, t in enumerate(tensors):
                 if t is not None:
                     ctypes.memmove(ctypes.addressof(view) + i * _TENSOR.size, ctypes.byref(_capi.tensor(t)), _TENSOR.size)
-        self.scalars.pack_into(raw, self.at, *scalars)
+        try:
+            self.scalars.pack_into(raw, self.at, *scalars)
+        except (struct.error, OverflowError) as e:
+            raise ValueError(f"lengths, windows and counts must be 32-bit integers, the softmax scale a float: {e}") from None
         return raw, view
 
 
@@ -272,7 +275,7 @@ def flash_attn_with_block_scaled_kvcache(
     if k_cache.ndim != 4 or block_table.ndim != 2 or cache_seqlens.ndim != 1:
         raise ValueError("caches must be [pages, page, heads, dim], block_table [batch, pages], cache_seqlens [batch]")
     if max_seqlen_k is None:
-        max_seqlen_k = block_table.shape[1] * k_cache.shape[1]
+        max_seqlen_k = min(block_table.shape[1] * k_cache.shape[1], 2 ** 31 - 1)
     if softmax_scale is None:
         softmax_scale = q.shape[-1] ** -0.5
     lib = _capi.library()

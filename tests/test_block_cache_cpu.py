@@ -127,3 +127,9 @@ def test_packed_copies_live_until_the_launch(monkeypatch):
     append_kvcache_block_scaled(x, x, cache, cache, scale, scale, torch.zeros(2, dtype=torch.int32),
                                 torch.zeros(2, 2, dtype=torch.int32), query=x)
     assert len(made) == 4 and all(alive) and len(alive) == 4
+
+
+@pytest.mark.parametrize("scalars", [(1, 2 ** 31, 0), (1, 2.5, 0), (1, None, 0), (-2 ** 31 - 1, 1, 0)])
+def test_numbers_that_do_not_fit_are_refused(scalars):
+    with pytest.raises(ValueError, match="32-bit"):
+        block_cache._APPEND.pack([None] * 15, scalars, 0)

@@ -718,7 +718,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (p.sinks)
           joined = join_sink(load_float(p.sinks, p.sink_t, h * p.si0) * 1.4426950408889634f, kOne * kUnit, m_run, l_run);
       }
-      const bool have = n_x > 0 && l_run > 0.f;
+      // Over a block-scaled cache a NaN sum stays one.
+      const bool some = BLOCK ? l_run != 0.f : l_run > 0.f, have = n_x > 0 && some;
       const float inv = have ? vscale * (joined * kUnit) / l_run : 0.f;
       const int wrow0 = (is_b ? it.row_b : it.row_a) + sub * 32;
       const bool staged = wrow0 + 32 <= it.q_len;  // warp-uniform
@@ -770,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           bulk_commit();
         }
       }
-      if (row_ok) p.lse[(int64_t)h * p.ls0 + t * p.ls1] = l_run > 0.f ? (m_run - kPBias<BF16, BLOCK> + log2f(l_run / kUnit)) * kLn2 : -INFINITY;
+      if (row_ok) p.lse[(int64_t)h * p.ls0 + t * p.ls1] = some ? (m_run - kPBias<BF16, BLOCK> + log2f(l_run / kUnit)) * kLn2 : -INFINITY;
     }
     if (lane == 0) bulk_wait_all();  // staged output stores complete before the CTA exits
   }

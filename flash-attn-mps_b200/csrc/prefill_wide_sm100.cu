@@ -559,7 +559,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
         if (p.sinks)
           joined = join_sink(load_float(p.sinks, p.sink_t, h * p.si0) * 1.4426950408889634f, kOne * kUnit, m_run, l_run);
       }
-      const bool have = n_x > 0 && l_run > 0.f;
+      // Over a block-scaled cache a NaN sum stays one.
+      const bool some = BLOCK ? l_run != 0.f : l_run > 0.f, have = n_x > 0 && some;
       const float inv = have ? vscale * (joined * kUnit) / l_run : 0.f;
       uint8_t* orow = reinterpret_cast<uint8_t*>(p.out) + (t * p.os0 + (int64_t)h * p.os1) * 2;
 #pragma unroll
@@ -580,7 +581,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
             *reinterpret_cast<uint4*>(orow + (c * 32 + v * 8) * 2) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
         }
       }
-      if (row_ok) p.lse[(int64_t)h * p.ls0 + t * p.ls1] = l_run > 0.f ? (m_run - kPBias<BF16, BLOCK> + log2f(l_run / kUnit)) * kLn2 : -INFINITY;
+      if (row_ok) p.lse[(int64_t)h * p.ls0 + t * p.ls1] = some ? (m_run - kPBias<BF16, BLOCK> + log2f(l_run / kUnit)) * kLn2 : -INFINITY;
     }
   }
   tc_fence_before();

@@ -253,3 +253,29 @@ def test_append_bounds_of_any_size(dtype, monkeypatch):
          max_seqlen=BIG)
     for t, want in zip((kc, vc, ks, vs), before):
         assert np.array_equal(base.np_of(t), want)
+
+
+@pytest.mark.parametrize("ns", [[1, 1], [4, 3], [130, 260]])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_nan_rows_stay_nan(dtype, ns):
+    """A NaN in a query or in a visible key makes exactly the rows that see it NaN, whatever kernel takes the call."""
+    heads, lens, d, at = (32, 4), [500, 300], 128, 299
+    if dtype == torch.float32 and max(ns) > 100:
+        heads, ns = (4, 2), [60, 40]
+    g = torch.Generator().manual_seed(3)
+    kc, vc, ks, vs, table = base.make_cache(g, lens, 16, 16, heads[1], d)
+    T = sum(ns)
+    q = torch.randn(T, heads[0], d, generator=g).to(dtype).cuda()
+    used, cu = torch.tensor(lens, dtype=torch.int32).cuda(), base.offsets(ns)
+    call = lambda: base.flash_attn_with_block_scaled_kvcache(
+        q, kc, vc, ks, vs, used, table, cu_seqlens_q=cu, max_seqlen_q=max(ns), max_seqlen_k=max(lens), return_softmax_lse=True)
+    want, want_lse = call()
+    q[0, 1, 7] = float("nan")
+    kc.view(torch.uint8)[table[1, at // 16].long(), at % 16, 0, 5] = 0x7f     # the last key of request 1, KV head 0
+    out, lse = call()
+    nan = torch.zeros(T, heads[0], dtype=torch.bool, device="cuda")
+    nan[0, 1] = True
+    nan[-1, :heads[0] // heads[1]] = True                                      # only the last query sees it
+    assert torch.equal(torch.isnan(out), nan[..., None].expand_as(out))
+    assert torch.equal(torch.isnan(lse), nan.T)
+    assert torch.equal(out[~nan], want[~nan]) and torch.equal(lse.T[~nan], want_lse.T[~nan])

@@ -279,3 +279,25 @@ def test_nan_rows_stay_nan(dtype, ns):
     assert torch.equal(torch.isnan(out), nan[..., None].expand_as(out))
     assert torch.equal(torch.isnan(lse), nan.T)
     assert torch.equal(out[~nan], want[~nan]) and torch.equal(lse.T[~nan], want_lse.T[~nan])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-25, 3.0])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_softmax_scales(dtype, scale):
+    """Scales that are zero, negative, tiny or large, for single tokens and prompt chunks."""
+    for ns, q_scale in (([1, 3], 1.0), ([130, 260], 1.0)):
+        g = torch.Generator().manual_seed(9)
+        lens = [300, 270]
+        kc, vc, ks, vs, table = base.make_cache(g, lens, 16, 16, 2, 128)
+        q = (torch.randn(sum(ns), 16, 128, generator=g) * q_scale).to(dtype).cuda()
+        used, cu = torch.tensor(lens, dtype=torch.int32).cuda(), base.offsets(ns)
+        out, lse = base.flash_attn_with_block_scaled_kvcache(
+            q, kc, vc, ks, vs, used, table, cu_seqlens_q=cu, max_seqlen_q=max(ns), max_seqlen_k=max(lens),
+            softmax_scale=scale, return_softmax_lse=True)
+        want, want_lse, spread = base.ob.attention(
+            base.np_of(q), [base.np_of(kc), base.np_of(vc)], [base.np_of(ks), base.np_of(vs)], lens, base.np_of(table),
+            base.np_of(cu), float(np.float32(scale)))
+        err = np.abs(lse.double().cpu().numpy() - want_lse)
+        assert (err <= 2e-5 + 2e-6 * np.abs(want_lse)).all(), err.max()
+        err = np.abs(out.double().cpu().numpy() - want)
+        assert (err <= base.EPS[dtype] * (np.abs(want) + spread) + 2e-5 * spread + 1e-7).all(), err.max()

@@ -903,6 +903,8 @@ __global__ void __launch_bounds__(128) block_merge_kernel(const DecodeArgs a, co
   if (col >= n * a.group) return;
   const int4 in = a.info[b * a.cblocks + cb];
   if (in.y <= in.x) return;  // one group holds the request: written already
+  // A decode that gave up on a wait may have left no such numbers.
+  if (in.x < 0 || in.y >= a.groups) return;
   const int D = p.c.D, pieces = in.y - in.x + 1;
   auto row_of = [&](int k) {
     const int64_t slot = 2 * (int64_t)(in.x + k) + (k == 0 && !in.z ? 1 : 0);

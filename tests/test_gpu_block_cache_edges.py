@@ -301,3 +301,63 @@ def test_softmax_scales(dtype, scale):
         assert (err <= 2e-5 + 2e-6 * np.abs(want_lse)).all(), err.max()
         err = np.abs(out.double().cpu().numpy() - want)
         assert (err <= base.EPS[dtype] * (np.abs(want) + spread) + 2e-5 * spread + 1e-7).all(), err.max()
+
+
+# Kernels and routes that sizes of real use reach, at small ones.
+@pytest.mark.parametrize("splits", [0, 2, 5, 60])
+@pytest.mark.parametrize("d", [128, 256])
+def test_sinks_over_joined_pieces(d, splits):
+    run_attention([1, 1, 0, 1], [2100, 700, 5, 0], 8, 2, d, 16, 16, torch.bfloat16, sinks=True, splits=splits)
+    run_attention([3, 1], [1500, 900], 8, 2, d, 32, 16, torch.float16, sinks=True, splits=splits, window=600, first=130)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prompt_chunks_in_several_passes(dtype, monkeypatch):
+    """A block table of 640000 tokens a request: the copies of two requests do not go into one pass."""
+    make = base.make_cache
+
+    def wide_table(*args, **kw):
+        *cache, table = make(*args, **kw)
+        return *cache, torch.cat([table, torch.full((table.shape[0], 40000), -1, dtype=torch.int32, device="cuda")], dim=1)
+    monkeypatch.setattr(base, "make_cache", wide_table)
+    run_prefill([130, 260, 17], [171, 300, 900], 32, 2, 128, 16, 16, dtype, max_k=640000, sinks=True)
+    run_prefill([130, 260, 17], [171, 300, 900], 32, 2, 128, 16, 16, dtype, max_k=640000, window=100, first=4,
+                mutate=lambda q, kc, vc, ks, vs, table: ks[:, :, 1].mul_(1.3))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_append_wide_heads_and_blocks(dtype):
+    """Units of 16 warps: blocks of 128 tokens with head dims above 128."""
+    for d, page in ((256, 128), (192, 256), (144, 128)):
+        base.run_append([200, 1, 131, 64], [0, 127, 70, 130], 4, 2, d, page, 128, dtype, seed=d)
+        base.run_append([17], [250], 4, 2, d, page, 128, dtype, seed=d, axes=3, interleaved=True)
+
+
+def test_verify_many_drafts():
+    """More drafts than a request's numbers in shared memory; all accepted, and rejected behind them."""
+    def accept(until):
+        def poke(logits, q, tokens, u, noise):
+            rows = list(range(100)) + list(range(101, 104))
+            tokens.copy_(logits[rows].argmax(-1))
+            u.fill_(0.5)
+            u[until] = 0.99999
+            logits[rows[until], 3] = logits[rows[until]].max()
+            logits[rows[until], 4] = logits[rows[until]].max()
+        return poke
+    for until in (0, 63, 64, 65, 99):
+        for temps in ([1e-3, 1.0], [0.0, 0.0]):
+            base.run_verify([100, 3], 61, torch.float32, one_hot=True, temps=temps, seed=2, poke=accept(until))
+
+
+def test_verify_more_rows_than_a_grid():
+    g = torch.Generator().manual_seed(4)
+    B, V = 40000, 3
+    logits = torch.randn(2 * B, V, generator=g).cuda() * 3
+    tokens = torch.randint(0, V, (B,), generator=g).cuda()
+    cu = torch.arange(B + 1, dtype=torch.int32).cuda()
+    u, noise = torch.rand(B, generator=g).cuda(), torch.empty(B, V).exponential_(generator=g).clamp_(min=1e-20).cuda()
+    got = base.verify_draft_tokens(logits, tokens, cu, u, noise, max_draft=1)
+    want, acc, _ = base.ob.verify(base.np_of(logits), base.np_of(tokens), base.np_of(cu), base.np_of(u), base.np_of(noise),
+                                  None, None, 1)
+    # Of 80000 random decisions about 80000 * 1e-6 may lie within float32's rounding.
+    assert (got[0].cpu().numpy() != want).any(1).sum() + (got[1].cpu().numpy() != acc).sum() <= 3

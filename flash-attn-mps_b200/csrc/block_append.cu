@@ -575,6 +575,7 @@ extern "C" int fa_append_block_scaled(const fa_block_append_args* g, void* strea
   for (int i = 0; i < 2; ++i) { a.xs0[i] = xs[i]->stride[0]; a.xs1[i] = xs[i]->stride[1]; a.xs2[i] = xs[i]->stride[2]; }
   if (present(g->query)) {
     FAB_CHECK_ARG(is_float(g->query.dtype), "query must be float");
+    FAB_CHECK_ARG(g->query.ndim == 3 && g->query.shape[1] >= 1, "query must have heads");
     if ((rc = check_rows(g->query, "query", T, a.c.D, g->query.dtype))) return rc;
     if ((rc = check_rows(g->query_out, "query_out", T, a.c.D, g->query.dtype))) return rc;
     FAB_CHECK_ARG(g->query_out.shape[1] == g->query.shape[1], "query_out must have the query's shape");

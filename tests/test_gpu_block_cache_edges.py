@@ -361,3 +361,13 @@ def test_verify_more_rows_than_a_grid():
                                   None, None, 1)
     # Of 80000 random decisions about 80000 * 1e-6 may lie within float32's rounding.
     assert (got[0].cpu().numpy() != want).any(1).sum() + (got[1].cpu().numpy() != acc).sum() <= 3
+
+
+def test_append_refuses_queries_without_heads():
+    g = torch.Generator().manual_seed(1)
+    kc, vc, ks, vs, table = base.make_cache(g, [64, 64], 16, 16, 2, 128)
+    used = torch.tensor([3, 9], dtype=torch.int32).cuda()
+    for new in (1, 600):
+        k = torch.randn(2, new, 2, 128, generator=g).to(torch.bfloat16).cuda()
+        with pytest.raises(ValueError, match="heads"):
+            base.append_kvcache_block_scaled(k, k, kc, vc, ks, vs, used, table, query=k[:, :, :0])

@@ -425,14 +425,23 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_pick_kernel(const Ve
     const int64_t drafted = i < n && !a.dp ? load_index(a.tok, a.tt, (int64_t)(begin + i) * a.tk0) : -1;
     const float is = 1.f / s;
     auto weight = [&](float x, float q, int v) { return fast_exp2((x - m) * k) * is - (v == drafted ? 1.f : q); };
-    auto divide = [&](int v) {
-      const float w = weight(V::one(a.x, row + v), with_q ? load_float(a.dp, a.dt, qrow + v) : 0.f, v);
-      best = max(best, quotient_key(w, a.noise[nrow + v], v));
+    auto read = [&](int v) { return weight(V::one(a.x, row + v), with_q ? load_float(a.dp, a.dt, qrow + v) : 0.f, v); };
+    auto divide = [&](int from, int to, int step) {
+#pragma unroll 1
+      for (int v = from; v < to; v += step) best = max(best, quotient_key(read(v), a.noise[nrow + v], v));
     };
-    // w / e by an approximate reciprocal, good to 2^-22 as w itself; by a division
-    // where that leaves float32's range.
+    // w / e by an approximate reciprocal, good to 2^-22 as w itself; false where
+    // that leaves float32's range and a division is due.
     float r = -1.f;
     int ri = 0x7fffffff;
+    auto approximate = [&](float w, float e, int v) {
+      float ie;
+      asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(ie) : "f"(e));
+      const float z = w * ie;
+      const bool in = z >= 0x1p-126f && z <= 0x1p100f;
+      if (in) rising(r, ri, z, v);
+      return in || !(w > 0.f);
+    };
     if (pl.y_vec) {
       for (int w0 = v0; w0 < v1; w0 += kPick * kVerifyThreads * N) {
         float x[kPick][N], y[kPick][N];
@@ -449,26 +458,18 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_pick_kernel(const Ve
           if (v < v1) {
             bool odd = false;
 #pragma unroll
-            for (int h = 0; h < N; ++h) {
-              const float w = weight(x[q][h], y[q][h], v + h);
-              float ie;
-              asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(ie) : "f"(e0[q][h]));
-              const float z = w * ie;
-              if (z >= 0x1p-126f && z <= 0x1p100f) rising(r, ri, z, v + h);
-              else odd |= w > 0.f;
-            }
-            if (odd) {
-#pragma unroll 1
-              for (int h = 0; h < N; ++h) divide(v + h);
-            }
+            for (int h = 0; h < N; ++h) odd |= !approximate(weight(x[q][h], y[q][h], v + h), e0[q][h], v + h);
+            if (odd) divide(v, v + N, 1);
           }
         }
       }
-      if (ri < a.V) best = max(best, quotient_key(r, ri));
     } else {
+      bool odd = false;
 #pragma unroll 4
-      for (int v = v0 + tid; v < v1; v += kVerifyThreads) divide(v);
+      for (int v = v0 + tid; v < v1; v += kVerifyThreads) odd |= !approximate(read(v), a.noise[nrow + v], v);
+      if (odd) divide(v0 + tid, v1, kVerifyThreads);
     }
+    if (ri < a.V) best = max(best, quotient_key(r, ri));
   }
   best = warp_max_key(best);
   if (lane == 0) {

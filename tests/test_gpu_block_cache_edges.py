@@ -371,3 +371,34 @@ def test_append_refuses_queries_without_heads():
         k = torch.randn(2, new, 2, 128, generator=g).to(torch.bfloat16).cuda()
         with pytest.raises(ValueError, match="heads"):
             base.append_kvcache_block_scaled(k, k, kc, vc, ks, vs, used, table, query=k[:, :, :0])
+
+
+@pytest.mark.parametrize("dtype,odd", [(torch.bfloat16, False), (torch.float16, True)])
+def test_prompt_chunks_in_a_cuda_graph(dtype, odd):
+    """A captured prompt chunk replayed over another cache content, with scales that both launches take: equal to eager calls."""
+    g = torch.Generator().manual_seed(6)
+    lens, ns = [300, 280], [130, 260]
+    kc, vc, ks, vs, table = base.make_cache(g, lens, 16, 16, 2, 128)
+    used, cu = torch.tensor(lens, dtype=torch.int32).cuda(), base.offsets(ns)
+    q = torch.randn(sum(ns), 32, 128, generator=g).to(dtype).cuda()
+
+    def step():
+        return base.flash_attn_with_block_scaled_kvcache(q, kc, vc, ks, vs, used, table, cu_seqlens_q=cu, max_seqlen_q=260,
+                                                         max_seqlen_k=300, return_softmax_lse=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in (1, 2):
+        h = torch.Generator().manual_seed(seed)
+        q.copy_(torch.randn(q.shape, generator=h).to(dtype))
+        if odd:
+            ks[:, :, seed - 1] *= 1.7
+        graph.replay()
+        got = [t.clone() for t in captured]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)

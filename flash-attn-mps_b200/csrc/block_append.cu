@@ -11,7 +11,8 @@
 // Bound by HBM (2 bytes read and 1 written per K/V element, 2 + 2 per Q element)
 // and, for the units, by instructions: 40928 tokens, 32/8 heads of 128, take
 // 105 us for Q (6.0 TB/s) and 95 for K and V (2.6 TB/s of 251 MB). One launch,
-// or two from kApart tokens on (one: 260 us together).
+// or two from kApart tokens on (one: 260 us together). The bf16 units are at their
+// cap of 128 registers and spill 4 bytes a thread.
 #include <algorithm>
 #include <type_traits>
 

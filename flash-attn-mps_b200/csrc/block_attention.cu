@@ -110,9 +110,14 @@ __global__ void __launch_bounds__(128) block_attention_any_kernel(const BlockAtt
 // ---- many query rows: a 16-bit copy of the visible rows, then the tcgen05 prefill
 //
 // Every prefill row block and head reads its keys again, so decoding them once
-// (1 byte read, 2 written per element: 30 us for 4 requests of 2500..8192 keys
-// with 8 KV heads of 128, in front of 575 us of prefill at 956 TFLOP/s)
-// turns the call into the 16-bit prefill's compute-bound work. block_mode_kernel
+// (1 byte read, 2 written per element: 29 us for 4 requests of 2500..8192 keys
+// with 8 KV heads of 128, in front of 560 us of prefill at 980 TFLOP/s)
+// turns the call into the 16-bit prefill's compute-bound work. As every 16-bit
+// prefill of the library it rounds P to q's type before P V (2^-9 for bf16, 2^-12
+// for f16; row sums keep float32): the tensor cores' 16-bit rate is what the
+// copy is made for, and P in two parts would double its P V products. The error
+// against 64 bits is 2.3e-3 of the output in bf16, 1.7e-3 of it from rounding
+// the output itself. block_mode_kernel
 // looks at the visible scales of every request and KV head first:
 //   0: code * scale is exact in the 16-bit type (4 significant bits): powers of
 //      two, in f16 up to 2^7 (448 * 2^7 = 57344) and K's from 2^-15 on. What
@@ -123,7 +128,8 @@ __global__ void __launch_bounds__(128) block_attention_any_kernel(const BlockAtt
 //      holds the codes alone and the prefill takes both scales as the formulas
 //      above do, one factor and one addend per key.
 // Rows in front of a window that share a tile with visible ones are written as
-// zeros, rows in tiles that no query sees not at all.
+// zeros, rows in tiles that no query sees not at all. The modes cost 4 us, the
+// launch over codes 3 where there is no head for it.
 struct CopyArgs {
   BlockCache c;
   uint16_t* k; uint16_t* v;          // [requests * max_k, HK, D]
@@ -386,9 +392,9 @@ int fill(const fa_block_attention_args* g, BlockAttn* p) {
 // 128 dims); the prefill 2.35 us on a tile of one item (a row block of 128
 // queries, of two heads where they pair), items in waves of one per SM, behind
 // the copy's 3 bytes per element. 8 requests, 32/8 heads, 8192 keys, measured
-// decode / copy and prefill: 16 queries 121 / 229 us, 32: 208 / 230, 48: 269 /
-// 230, 128: 696 / 231; one request: 64 queries 72 / 159, 256: 202 / 160; head
-// dim 256, 4 requests: 32 queries 167 / 214, 64: 275 / 213.
+// decode / copy and prefill: 16 queries 99 / 231 us, 32: 187 / 231, 48: 255 /
+// 231, 128: 701 / 231; one request: 64 queries 58 / 163, 256: 185 / 163; head
+// dim 256, 4 requests: 32 queries 131 / 219, 64: 234 / 219.
 bool prefill_pays(const BlockAttn& p) {
   if (p.max_q < 16) return false;
   const int block = block_decode_columns(p), cols = p.max_q * (p.HQ / p.c.HK);

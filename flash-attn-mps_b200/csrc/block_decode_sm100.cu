@@ -44,13 +44,15 @@
 // 16-token pages make 16 boxes a tile, and one warp issued them at 4.2 TB/s).
 // Rings decouple them, so the gathers run on into the next request.
 // HBM-bound: D bytes of K and of V per key and KV head, once for all columns.
-// 32 requests x 32768 tokens, 32/8 heads of 128, 16-token pages: 347 us, 6.2 TB/s
-// of K and V (page 64: 6.5); the library's mma.sync decode of a cache with one
+// 32 requests x 32768 tokens, 32/8 heads of 128, 16-token pages: 348 us, 6.2 TB/s
+// of K and V (page 64: 330, 6.5); the library's mma.sync decode of a cache with one
 // descale per head takes 428. More columns are bound by the softmax warps: 8192
-// tokens, 4 / 8 / 16 / 24 / 32 columns a KV head 94 / 99 / 125 / 154 / 171 us
-// (bf16; f16 with its third part 100 / 132 / 164 / 188 for 8 to 32), issue slots
-// 54 % busy. Their arithmetic goes two columns to an instruction (f32x2; column
-// by column 137 / 159 / 177 for 16 to 32).
+// tokens, 4 / 8 / 16 / 24 / 32 columns a KV head 96 / 110 / 133 / 183 / 198 us
+// (bf16; f16 with its fourth part 96 / 109 / 138 / 185 / 203) one call behind
+// another. Their arithmetic goes two columns to an instruction (f32x2; column
+// by column 6 % slower at 16 to 32 columns). Prompts of 32-column blocks alone
+// are 5 to 9 % slower than with two E4M3 parts. Of the shapes bf16 rows of 256
+// with 32 columns spill 16 bytes.
 //
 // Every wait is bounded; on a timeout the CTA records a flag, drains its own
 // copies and MMAs, frees tensor memory and returns.
@@ -68,11 +70,6 @@ namespace fab {
 namespace {
 
 using namespace sm100;
-using pf::fadd2;
-using pf::ffma2;
-using pf::fmul2;
-using pf::f2pack;
-using pf::f2unpack;
 using pf::fadd2;
 using pf::ffma2;
 using pf::fmul2;

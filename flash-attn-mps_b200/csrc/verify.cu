@@ -11,9 +11,11 @@
 // statistics (a few numbers), walk the acceptance chain and search their chunk
 // of the row it names; the last CTA of a request writes its tokens. The second
 // launch may begin before the first ends and waits for it on the device.
-// 64 requests of 1..5 drafts, 151936 tokens, bf16: 44 us for 154 MB (3.5 TB/s),
-// 24 and 26 us by themselves: latency (the chain statistics -> acceptance -> row)
+// 64 requests of 1..5 drafts, 151936 tokens, bf16: 45 us for 154 MB (3.4 TB/s),
+// 19 and 27 us by themselves: latency (the chain statistics -> acceptance -> row)
 // before bandwidth. One request: 19 us a call, the host's time; 12 on the GPU.
+// Weights and their quotients are good to a few units of float32; of two that
+// lie closer together either may be taken, whichever route a call goes.
 #include <algorithm>
 
 #include "common.cuh"

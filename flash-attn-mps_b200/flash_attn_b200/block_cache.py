@@ -15,7 +15,7 @@ needed before the first token. One step of a (speculative) decoder calls
 * ``verify_draft_tokens``: keep the drafted tokens that the target accepts and
   sample the one behind them.
 
-Arguments are checked by the CUDA library (``ValueError``); every call is
+Arguments are checked before the launch (``ValueError``); every call is
 asynchronous on the current stream and reads no tensor value on the host, so a
 step can be captured in a CUDA graph. Inference only.
 """
@@ -252,6 +252,11 @@ def flash_attn_with_block_scaled_kvcache(
     -inf. ``max_seqlen_k`` bounds ``cache_seqlens`` (default: what the block
     table holds); it sizes the launch and reads no tensor.
 
+    Scores, maxima and sums are float32. Probabilities are rounded to 2^-9 of
+    their value for bfloat16 queries and 2^-12 for float16, down to 20 nats
+    below the largest in reach (prompt chunks in float16: 14); float32 queries
+    keep them in float32.
+
     Returns ``out`` (q's shape and dtype), with ``return_softmax_lse`` also the
     natural-log LSE: ``[heads, tokens]``, or ``[batch, heads, queries]`` for a
     4-D ``q``.
@@ -305,7 +310,9 @@ def verify_draft_tokens(target_logits, draft_tokens, cu_seqlens_draft, uniform, 
     where that is zero throughout) and ``p`` after the last draft: with
     ``noise`` drawn from Exp(1), a sample of ``w``, so that the tokens follow
     the target's distribution. ``uniform`` is float32 ``[drafts]`` in [0, 1),
-    ``noise`` float32 ``[batch, vocabulary]``, positive.
+    ``noise`` float32 ``[batch, vocabulary]``, positive. Probabilities and
+    quotients are float32: of decisions that lie within a few units of its
+    rounding either may be taken.
 
     Returns ``tokens`` (int64 ``[batch, max_draft + 1]``, -1 behind the last)
     and ``accepted`` (int32 ``[batch]``).

@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(256) block_copy_kernel(const CopyArgs a) {
     const int r = e / per_row, rem = e - r * per_row, h = rem / per_head, d = (rem - h * per_head) * 16;
     const int t = t0 + r;
     const bool codes = a.mode[(int64_t)lb * c.HK + h];
-    if (t >= len && !codes) break;
+    if (t >= len && !codes) continue;  // another head's scales may still be due
     uint4 kv[2];
     float s[2];
     const bool seen = pg >= 0 && t < len && (t >= lo || t < a.first);
@@ -312,7 +312,7 @@ int launch_prefill(const BlockAttn& p, const Plan& plan, void* workspace, cudaSt
     a.cu_q = p.cu_q; a.cq0 = p.cq0;
     a.used = p.used; a.u0 = p.u0;
     a.b0 = b0; a.B = n; a.max_k = p.max_k; a.win = p.win; a.first = p.first;
-    const dim3 grid((unsigned)((p.max_k + 15) / 16), (unsigned)n);
+    const dim3 grid((unsigned)(kfac_stride(p) / 16), (unsigned)n);  // whole key tiles
     const dim3 heads((unsigned)p.c.HK, (unsigned)n);
     if (p.qt == FA_BF16) block_mode_kernel<true><<<heads, 256, 0, st>>>(a);
     else block_mode_kernel<false><<<heads, 256, 0, st>>>(a);

@@ -402,3 +402,35 @@ def test_prompt_chunks_in_a_cuda_graph(dtype, odd):
         got = [t.clone() for t in captured]
         for a, b in zip(got, step()):
             assert torch.equal(a, b)
+
+
+@pytest.fixture
+def poisoned_workspaces(monkeypatch):
+    """Workspaces and outputs begin as NaN in every type."""
+    new_empty = torch.Tensor.new_empty
+
+    def poisoned(self, *args, **kw):
+        t = new_empty(self, *args, **kw)
+        if t.numel():
+            t.view(torch.uint8).fill_(0xff)
+        return t
+    monkeypatch.setattr(torch.Tensor, "new_empty", poisoned)
+
+
+@pytest.mark.parametrize("hk,d", [(1, 48), (2, 48), (3, 48), (3, 128), (5, 80), (3, 208)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_nothing_left_in_workspaces_is_read(dtype, hk, d, poisoned_workspaces):
+    """Ends of requests inside a tile, heads of both scale forms side by side, pieces and merges, over poisoned memory."""
+    def mutate(q, kc, vc, ks, vs, table):
+        ks[:, :, 0] *= 1.3
+    for mutation in (None, mutate):
+        run_prefill([130, 260], [171, 300], 32 // hk * hk, hk, d, 16, 16, dtype, mutate=mutation)
+        run_prefill([260, 130], [900, 131], 32 // hk * hk, hk, d, 16, 16, dtype, mutate=mutation, window=200, first=130)
+    for splits in (0, 1, 3, 40):
+        run_attention([1, 0, 1, 2], [171, 9, 1300, 5], 2 * hk, hk, d, 16, 16, dtype, mutate=mutate, splits=splits)
+        run_attention([1, 0, 1, 2], [171, 9, 1300, 5], 2 * hk, hk, d, 16, 16, dtype, splits=splits, window=300, first=5)
+
+
+def test_verification_reads_nothing_left_in_its_workspace(poisoned_workspaces):
+    for V in (1, 1000, 4097, 151936):
+        base.run_verify([3, 0, 1, 5, 2], V, torch.bfloat16, temps=[0.7, 1.0, 0.0, 1.3, 0.0], seed=11 + V)

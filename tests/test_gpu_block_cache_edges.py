@@ -434,3 +434,108 @@ def test_nothing_left_in_workspaces_is_read(dtype, hk, d, poisoned_workspaces):
 def test_verification_reads_nothing_left_in_its_workspace(poisoned_workspaces):
     for V in (1, 1000, 4097, 151936):
         base.run_verify([3, 0, 1, 5, 2], V, torch.bfloat16, temps=[0.7, 1.0, 0.0, 1.3, 0.0], seed=11 + V)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_append_behind_any_scales_and_positions(dtype, monkeypatch):
+    """Older scales that are no powers of two; positions in front of and behind the tables."""
+    make = base.make_cache
+
+    def scaled(*args, **kw):
+        kc, vc, ks, vs, table = make(*args, **kw)
+        return kc, vc, ks * 1.375, vs * 0.8125, table
+    monkeypatch.setattr(base, "make_cache", scaled)
+    base.run_append([9, 33, 1, 130], [5, 10, 31, 17], 6, 2, 128, 32, 16, dtype, scale=8.0)
+    base.run_append([9, 33, 1, 130], [5, 10, 31, 17], 6, 2, 128, 64, 64, dtype, scale=0.1)
+    call = base.append_kvcache_block_scaled
+
+    def shifted(*args, positions, **kw):
+        assert (positions < 0).any() and (positions >= kw["rotary_cos"].shape[0]).any()
+        return call(*args, positions=positions, **kw)
+    monkeypatch.setattr(base, "append_kvcache_block_scaled", shifted)
+    randint = torch.randint
+    monkeypatch.setattr(torch, "randint", lambda lo, hi, *a, **kw: randint(lo - 50 if kw.get("dtype") == torch.int32 else lo,
+                                                                           hi + 50 if kw.get("dtype") == torch.int32 else hi, *a, **kw))
+    base.run_append([9, 33, 90], [5, 10, 17], 6, 2, 128, 32, 16, dtype)
+    base.run_append([9, 33, 90], [5, 10, 17], 6, 2, 128, 32, 16, dtype, axes=3)
+
+
+def strided_copy(x, dims):
+    """x's values with other strides: dimensions stored in the order `dims`, two elements apart."""
+    out = torch.zeros(*[x.shape[i] for i in dims], 2, dtype=x.dtype, device=x.device)[..., 1]
+    out = out.permute(*[dims.index(i) for i in range(x.ndim)])
+    return out.copy_(x)
+
+
+def heads_first(cache):
+    """A cache stored heads before tokens."""
+    raw = cache.view(torch.uint8).permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+    return raw.view(torch.float8_e4m3fn)
+
+
+@pytest.mark.parametrize("ns", [[1, 1], [5, 3], [130, 260]])
+def test_strided_scales_tables_and_lengths(ns):
+    """Every small tensor strided, K and V caches of different layouts: equal to the contiguous call."""
+    g = torch.Generator().manual_seed(2)
+    lens = [500, 300]
+    kc, vc, ks, vs, table = base.make_cache(g, lens, 32, 16, 2, 128)
+    q = torch.randn(sum(ns), 16, 128, generator=g).to(torch.bfloat16).cuda()
+    k, v = torch.randn(2, sum(ns), 2, 128, generator=g).to(torch.bfloat16).cuda()
+    starts = torch.tensor(lens, dtype=torch.int32).cuda() - torch.tensor(ns, dtype=torch.int32).cuda()
+    used, cu = torch.tensor(lens, dtype=torch.int32).cuda(), base.offsets(ns)
+    angle = torch.rand(600, 64, generator=g).cuda()
+    cos, sin, pos = angle.cos(), angle.sin(), torch.randint(0, 600, (sum(ns),), generator=g, dtype=torch.int32).cuda()
+    aux = torch.randn(16, generator=g).cuda()
+
+    def step(kc, vc, ks, vs, table, starts, used, cu, cos, sin, pos, aux):
+        r = base.append_kvcache_block_scaled(k, v, kc, vc, ks, vs, starts, table, cu_seqlens=cu, max_seqlen=max(ns), query=q,
+                                             rotary_cos=cos, rotary_sin=sin, positions=pos)
+        return r, *base.flash_attn_with_block_scaled_kvcache(r, kc, vc, ks, vs, used, table, cu_seqlens_q=cu, max_seqlen_q=max(ns),
+                                                             max_seqlen_k=500, s_aux=aux, return_softmax_lse=True), kc, vc, ks, vs
+    contiguous = (kc.clone(), vc.clone(), ks.clone(), vs.clone(), table, starts, used, cu, cos, sin, pos, aux)
+    strided = (kc, heads_first(vc), strided_copy(ks, (2, 0, 1)), strided_copy(vs, (1, 2, 0)), strided_copy(table, (1, 0)),
+               *[strided_copy(t, (0,)) for t in (starts, used, cu)], strided_copy(cos, (0, 1)), strided_copy(sin, (1, 0)),
+               strided_copy(pos, (0,)), strided_copy(aux, (0,)))
+    for a, b in zip(step(*contiguous), step(*strided)):
+        if a.dtype == torch.float8_e4m3fn:
+            a, b = a.view(torch.uint8), b.view(torch.uint8)
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("ns", [[1, 1], [130, 260]])
+def test_offsets_past_32_bits(ns):
+    """Pages more than 2^31 bytes into the cache: equal to the same pages in a small one."""
+    g = torch.Generator().manual_seed(2)
+    lens, page, hk, d = [500, 300], 128, 8, 128
+    small = base.make_cache(g, lens, page, 128, hk, d)
+    pages = 2 ** 31 // (page * hk * d) + 20
+    far = pages - small[0].shape[0]
+    big = [torch.zeros(pages, page, hk, d, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2)]
+    big += [torch.ones(pages, 1, hk, device="cuda") for _ in range(2)]
+    for x, y in zip(big, small):
+        x.view(torch.uint8)[far:].copy_(y.view(torch.uint8))
+    table = torch.where(small[4] >= 0, small[4] + far, -1)
+    q = torch.randn(sum(ns), 32, d, generator=g).to(torch.bfloat16).cuda()
+    k, v = torch.randn(2, sum(ns), hk, d, generator=g).to(torch.bfloat16).cuda()
+    used, cu = torch.tensor(lens, dtype=torch.int32).cuda(), base.offsets(ns)
+    starts = used - torch.tensor(ns, dtype=torch.int32).cuda()
+    got = []
+    for cache, t in ((big, table), (small[:4], small[4])):
+        base.append_kvcache_block_scaled(k, v, *cache, starts, t, cu_seqlens=cu, max_seqlen=max(ns))
+        got.append(base.flash_attn_with_block_scaled_kvcache(q, *cache, used, t, cu_seqlens_q=cu, max_seqlen_q=max(ns),
+                                                             max_seqlen_k=500, return_softmax_lse=True))
+        got[-1] += tuple(x.view(torch.uint8)[far if cache is big else 0:] for x in cache)
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+def test_verify_offsets_past_32_bits():
+    g = torch.Generator().manual_seed(3)
+    V, stride = 1024, 3 * 2 ** 29
+    want = torch.randn(4, V, generator=g).to(torch.bfloat16).cuda()
+    logits = torch.empty(3 * stride + V, dtype=torch.bfloat16, device="cuda").as_strided((4, V), (stride, 1))
+    logits.copy_(want)
+    tokens = torch.randint(0, V, (2,), generator=g).cuda()
+    u, noise = torch.rand(2, generator=g).cuda() * 1e-4, torch.rand(2, V, generator=g).cuda() + 0.01
+    calls = [base.verify_draft_tokens(x, tokens, base.offsets([2, 0]), u, noise, max_draft=2) for x in (logits, want)]
+    assert all(torch.equal(a, b) for a, b in zip(*calls))

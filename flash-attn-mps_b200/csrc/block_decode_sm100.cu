@@ -14,7 +14,8 @@
 //     columns of the same MMA (N = 16 is its least width).
 //   * P becomes a sum of E5M2 parts, part i scaled by 2^(3 i): 3 parts for bf16
 //     hold a probability to 2^-9, as the 16-bit type itself would, 4 for f16 to
-//     2^-12, down to 2^-29 of the tile's largest (20 nats); below that the error
+//     2^-12, down to 2^-29 of the tile's largest (20 nats; of p vs, which is what
+//     the tile's maximum is taken of); below that the error
 //     stays under 2^-38 (2^-41) of the largest. The wide exponent matters where
 //     the largest keys add nothing to an output (an attention sink's V row is
 //     close to zero): E4M3 parts, which hold 2^-14, lost such rows.

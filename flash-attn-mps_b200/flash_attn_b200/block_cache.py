@@ -254,8 +254,8 @@ def flash_attn_with_block_scaled_kvcache(
 
     Scores, maxima and sums are float32. Probabilities are rounded to 2^-9 of
     their value for bfloat16 queries and 2^-12 for float16, down to 20 nats
-    below the largest in reach (prompt chunks in float16: 14); float32 queries
-    keep them in float32.
+    below the largest in reach (prompt chunks in float16: 14), each taken with
+    its V block's scale; float32 queries keep them in float32.
 
     Returns ``out`` (q's shape and dtype), with ``return_softmax_lse`` also the
     natural-log LSE: ``[heads, tokens]``, or ``[batch, heads, queries]`` for a

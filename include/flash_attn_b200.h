@@ -364,7 +364,8 @@ int fa_append_block_scaled(const fa_block_append_args* args, void* stream);
  * tile sees never enter a product. s_aux adds one logit per head to the
  * denominator. num_splits 0 lets the library choose. Probabilities are rounded
  * to 2^-9 (bf16 q) or 2^-12 (f16 q) of their value down to 20 nats below the
- * largest in reach (14 for prompt chunks in f16). max_seqlen_q and
+ * largest in reach (14 for prompt chunks in f16), each taken with its V block's
+ * scale. max_seqlen_q and
  * max_seqlen_k may be any upper bounds; requests hold less than 2^30 tokens.
  */
 typedef struct fa_block_attention_args {

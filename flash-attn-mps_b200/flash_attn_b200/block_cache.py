@@ -257,6 +257,9 @@ def flash_attn_with_block_scaled_kvcache(
     below the largest in reach (prompt chunks in float16: 14), each taken with
     its V block's scale; float32 queries keep them in float32.
 
+    A NaN in a query or in a visible K makes the rows that see it NaN; one in V
+    its element of these rows and of those computed in a tile with them.
+
     Returns ``out`` (q's shape and dtype), with ``return_softmax_lse`` also the
     natural-log LSE: ``[heads, tokens]``, or ``[batch, heads, queries]`` for a
     4-D ``q``.

@@ -361,7 +361,10 @@ int fa_append_block_scaled(const fa_block_append_args* args, void* stream);
  * dtype, lse [Hq,T] f32. Query position i sees key j when j <= i (causal) and,
  * with window_left >= 0, when also i - j <= window_left or j < first_tokens.
  * Rows that see no key give 0 and -inf; rows of K and V that no query of a
- * tile sees never enter a product. s_aux adds one logit per head to the
+ * tile sees never enter a product. A NaN in a query or in a visible row of K
+ * makes exactly the rows of out that see it NaN; a NaN in V makes its element NaN
+ * also in rows that are computed in one tile with a row that sees it (drafted
+ * tokens of a request, 128 queries of a prompt). s_aux adds one logit per head to the
  * denominator. num_splits 0 lets the library choose. Probabilities are rounded
  * to 2^-9 (bf16 q) or 2^-12 (f16 q) of their value down to 20 nats below the
  * largest in reach (14 for prompt chunks in f16), each taken with its V block's
